@@ -18,7 +18,7 @@ z.  Slots go in blocks of 32; with n = ceil(head_dim / 32) (missing values have 
   128 n words of value codes  [piece][g = 0..3][m = 0..15][e]: the word of dimension d = 16 (piece E + e) + m
                               holds tokens 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3 (E = 4 for even n, else 2)
   32 words of key scales, 32 words of value scales
-and in a word of eight codes, code j lies at bit 4 (j // 2) + 16 (j % 2).
+and in a word of eight codes, code j takes four bits from bit 2 + 4 (j // 2) + 16 (j % 2) on, bit 32 being bit 0 again.
 """
 import math
 import os
@@ -182,13 +182,24 @@ def _shifts(device):
     return 4 * (j // 2) + 16 * (j % 2)
 
 
+def _turned(w):
+    """Words two bits to the left, the top two at the bottom."""
+    return (w << 2) | ((w >> 30) & 3)
+
+
 def _join(c):
     """Eight codes along the last axis -> one word."""
-    return (c.to(torch.int32) << _shifts(c.device)).sum(-1, dtype=torch.int32)
+    return _turned((c.to(torch.int32) << _shifts(c.device)).sum(-1, dtype=torch.int32))
 
 
 def _split(w):
+    w = ((w >> 2) & 0x3FFFFFFF) | (w << 30)
     return (w[..., None] >> _shifts(w.device)) & 15
+
+
+def _one(w, shift):
+    """The code of each word that lies `shift` + 2 bits up."""
+    return ((((w >> 2) & 0x3FFFFFFF) | (w << 30)) >> shift) & 15
 
 
 def _pages_of(kc, kw, vc, vw):
@@ -364,13 +375,13 @@ def _append(st):
     tile, m = dd // 16, dd % 16
     g, j = tok % 16 // 4, tok % 4 + 4 * (tok // 16)
     at = 128 * n + ((tile // e) * 64 + g[..., None] * 16 + m) * e + tile % e                # [rows, 1, d]
-    sh = (4 * (j // 2) + 16 * (j % 2))[..., None]
+    sh = (4 * (j // 2) + 16 * (j % 2))[..., None].int()
     idx = (pg[..., None], h[:, None], blk[..., None], at)
-    old = (w[idx] >> sh) & 15
-    w.index_put_(idx, ((vc - old) << sh).int(), accumulate=True)
+    old = _one(w[idx], sh)
+    w.index_put_(idx, _turned(vc << sh) - _turned(old << sh), accumulate=True)
     # and the tokens' values back
     k = _split(w[pg[..., None], h[:, None], blk[..., None], tok[..., None] * (4 * n) + torch.arange(4 * n, device=pg.device)])
-    v = (w[idx] >> sh) & 15
+    v = _one(w[idx], sh)
     return (_value(k.reshape(-1, heads, 32 * n)[..., :d], w[pg, h, blk, 256 * n + tok]).to(st["dtype"]),
             _value(v, w[pg, h, blk, 256 * n + 32 + tok]).to(st["dtype"]))
 
