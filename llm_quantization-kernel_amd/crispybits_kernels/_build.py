@@ -25,7 +25,8 @@ ARCH = os.environ.get("CRISPYBITS_ARCH", "gfx950")
 
 SOURCES = ["abi.cpp", "gemv_stream.hip", "gemv_bsub.hip", "gemv_any.hip", "gemm.hip", "gemm_f16.cpp", "gemm_f16_mb1.hip",
            "gemm_f16_mb2.hip", "gemm_f16_mb4.hip", "gemm_f16_mb4s.hip", "gemm_f32.hip",
-           "unpack.hip", "quant.hip", "probe.hip"]
+           "unpack.hip", "quant.hip", "probe.hip", "attn_abi.cpp", "kv4_store.hip", "kv4_attn.hip", "prompt_attn.hip",
+           "prompt_attn_f32.hip"]
 
 # -packed-fp32-ops is disabled: the kernels never rely on v_pk_*_f32.
 HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-fp-atomics",
@@ -55,7 +56,7 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
-EXT_SOURCE = "torch_ext.cpp"
+EXT_SOURCES = ["torch_ext.cpp", "torch_attn.cpp"]
 
 
 def _ext_path() -> str:
@@ -80,16 +81,16 @@ def _torch_flags():
     return [f"-I{p}" for p in inc] + defs, libs
 
 
-def _compile_ext(verbose: bool) -> str:
-    obj = os.path.join(OBJ_DIR, "torch_ext.o")
+def _compile_ext(src: str, verbose: bool) -> str:
+    obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
     cflags, _ = _torch_flags()
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-w", *cflags, "-c",
-           os.path.join(CSRC, EXT_SOURCE), "-o", obj]
+           os.path.join(CSRC, src), "-o", obj]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"compile failed for {EXT_SOURCE}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"compile failed for {src}:\n{r.stdout}\n{r.stderr}")
     return obj
 
 
@@ -105,17 +106,17 @@ def build(verbose: bool = False) -> str:
     """Compile every HIP/C++ source, link the C-ABI library and the torch op module over it;
     returns the library's path."""
     os.makedirs(OBJ_DIR, exist_ok=True)
-    jobs = min(len(SOURCES) + 1, max(1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 4))))
+    jobs = min(len(SOURCES) + len(EXT_SOURCES), max(1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 4))))
     with ThreadPoolExecutor(jobs) as ex:
-        ext_obj = ex.submit(_compile_ext, verbose)
+        ext_objs = [ex.submit(_compile_ext, s, verbose) for s in EXT_SOURCES]
         objs = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
-        ext_obj = ext_obj.result()
+        ext_objs = [o.result() for o in ext_objs]
     tmp = LIB_PATH + ".tmp"
     _run([_hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}", *objs, "-o", tmp], verbose, "link")
     os.replace(tmp, LIB_PATH)
     _, libs = _torch_flags()
     ext = _ext_path()
-    _run([os.environ.get("CXX", "g++"), "-shared", "-fPIC", ext_obj, "-o", ext + ".tmp", f"-L{PKG_DIR}",
+    _run([os.environ.get("CXX", "g++"), "-shared", "-fPIC", *ext_objs, "-o", ext + ".tmp", f"-L{PKG_DIR}",
           "-lcrispybits_hip", "-Wl,-rpath,$ORIGIN", *libs], verbose, "extension link")
     os.replace(ext + ".tmp", ext)
     return LIB_PATH

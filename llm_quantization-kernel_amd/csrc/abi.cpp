@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "crispybits_hip.h"
+#include "cbk_host.hpp"
 #include "cbk_kernels.hpp"
 
 using namespace cbk;
@@ -57,6 +58,10 @@ namespace {
 
 thread_local std::string g_err;
 
+}  // namespace
+
+namespace cbk {
+
 int fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
@@ -71,20 +76,9 @@ int hip_fail(hipError_t e, const char* what) {
     return fail(CBK_EHIP, "%s: %s", what, hipGetErrorString(e));
 }
 
-// Switches to `device` for the duration of a call (the reference's CUDAGuard).
-struct DeviceGuard {
-    int prev = -1;
-    hipError_t err = hipSuccess;
-    explicit DeviceGuard(int device) {
-        err = hipGetDevice(&prev);
-        if (err == hipSuccess && prev != device) err = hipSetDevice(device);
-        else if (err != hipSuccess) prev = -1;
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
-    }
-};
+}  // namespace cbk
+
+namespace {
 
 constexpr int MAX_DEVICES = 64;
 int g_cu[MAX_DEVICES];
@@ -138,13 +132,11 @@ hipError_t scratch_for(int device, float** out) {
 // flight).  A call that finds no window of its own and no free one, or whose row blocks
 // outnumber a window's counters, takes the combine launch instead: correct, one launch
 // more.  So does a call on hipStreamPerThread, one handle for a stream of each thread.
-// One graph must not be replayed while another replay of it runs.  Decode calls and
-// prefill GEMMs have windows of their own (WIN_DECODE, WIN_GEMM): a program that captures
-// a graph per prompt length leaves its decode graphs theirs.
-enum { WIN_DECODE = 0, WIN_GEMM = 1 };
+// One graph must not be replayed while another replay of it runs.  Decode calls,
+// prefill GEMMs and cache attention have windows of their own (WIN_DECODE, WIN_GEMM,
+// WIN_ATTN): a program that captures a graph per prompt length leaves its decode graphs theirs.
 constexpr int SPLIT_WINDOWS = 256;
-constexpr int SPLIT_COUNTERS = 4096;
-static __device__ __align__(256) uint32_t split_counters[2 * SPLIT_WINDOWS * SPLIT_COUNTERS];
+static __device__ __align__(256) uint32_t split_counters[WIN_KINDS * SPLIT_WINDOWS * SPLIT_COUNTERS];
 
 struct SplitWindows {
     std::mutex mu;
@@ -156,10 +148,10 @@ struct SplitWindows {
     hipStream_t stream[SPLIT_WINDOWS];              // holder stream
     unsigned long long capture[SPLIT_WINDOWS];      // and its capture's id (capture windows)
 };
-SplitWindows g_split[2][MAX_DEVICES];
+SplitWindows g_split[WIN_KINDS][MAX_DEVICES];
 
 // The counter window of this call on `device` (made current by the caller), or nullptr.
-// kind: WIN_DECODE or WIN_GEMM.
+// kind: WIN_DECODE, WIN_GEMM or WIN_ATTN.
 uint32_t* split_window(int kind, int device, hipStream_t stream) {
     if (device < 0 || device >= MAX_DEVICES || stream == hipStreamPerThread) return nullptr;
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
@@ -776,6 +768,7 @@ int run_gemm_f16(GemmArgs& A, int dtype, int mode, float* partial, int64_t parti
 
 namespace cbk {
 hipError_t lds_limit_raise(const void* f, int bytes) { return ensure_lds(f, bytes); }
+uint32_t* attn_window(int device, hipStream_t stream) { return split_window(WIN_ATTN, device, stream); }
 }  // namespace cbk
 
 extern "C" {

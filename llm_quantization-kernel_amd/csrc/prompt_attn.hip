@@ -1,0 +1,309 @@
+// prompt_attn.hip -- causal attention over packed prompts, fp16 / bf16, on the 16-bit matrix cores.
+//
+// Row i of a sequence sees its rows 0 .. i; query head h reads kv head h / group.  One pass over the keys with
+// the running maximum and sum of the softmax: per tile of 64 tokens
+//   S^T[token, row] = K q^T,  w = 2^(scale log2e S - M),  O^T[d, row] += V^T w
+// A workgroup has 128 rows of one head (32 a wave) and stages K and V tiles in LDS, the next tile's loads under
+// way.  v_mfma_f32_32x32x16 gives a lane one row's column of S^T (tokens 8 i + 4 (lane / 32) + 0..3), which is the
+// operand layout of w for the tokens in that order, so w stays in its lane; V^T is read transposed from LDS
+// (ds_read_b64_tr_b16) in the same token order.  The running reference M of a row moves only when a tile's
+// largest score exceeds it by 8 (w < 2^8 then, in range of fp16; sums are fp32).
+//
+// Masked places take no part whatever they hold: scores there are selected away, and a V tile on the diagonal
+// that has infinities or NaN (a product 0 x inf would reach rows that do not see it) is taken with those values
+// zeroed, and what a row sees of them is added at the end.
+#include "kv4.hpp"
+#include "cbk_kernels.hpp"
+
+namespace cbk {
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int WAVES = 4;
+constexpr int ROWS = 32 * WAVES;       // query rows of a workgroup
+constexpr int KT = 64;                 // tokens of a tile
+constexpr float LOW = -1e30f;
+constexpr float SLACK = 8.f;
+
+template <int DT>
+__device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
+    if constexpr (DT == DT_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// Two values rounded to the type (nearest even), packed.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    if constexpr (DT == DT_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
+    }
+}
+
+__device__ __forceinline__ f16v zero16() {
+    f16v z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* glb_ptr;
+
+// Position (in 16-byte chunks) of chunk c of row r in a tile of CP chunks a row.  K: a wave's reads take two
+// neighbouring chunks of 32 rows; V: four neighbouring chunks of eight rows.  Both orders spread them over the banks.
+template <int CP>
+__device__ __forceinline__ int k_at(int r, int c) { return r * CP + (c ^ (r & (CP - 1))); }
+template <int CP>
+__device__ __forceinline__ int v_at(int r, int c) { return r * CP + (c ^ ((r & 3) << 2 & (CP - 1))); }
+
+// KS: steps of 16 of the head's values, DT32: tiles of 32, CP: chunks of a row in LDS.
+template <int DT, int KS, int CP>
+__global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kernel(PromptArgs A, int row_tiles) {
+    constexpr int DT32 = (KS + 1) / 2;
+    constexpr int TILE = KT * CP * 16;                 // bytes of a K or V tile
+    auto not_finite = [](uint32_t v) {                 // all ones in each 16-bit half that is an infinity or NaN
+        constexpr uint32_t EX = DT == DT_F16 ? 0x7C00u : 0x7F80u;
+        return ((v & EX) == EX ? 0xFFFFu : 0u) | ((v >> 16 & EX) == EX ? 0xFFFF0000u : 0u);
+    };
+    extern __shared__ __align__(16) char lds[];        // [2][K tile, V tile]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, hf = lane >> 5;
+
+    // kv heads innermost: with the workgroups dealt out to the XCDs in turn, a kv head's tiles stay on one; the
+    // longest rows' tiles first
+    int id = blockIdx.x;
+    const int hk = id % A.hkv;
+    id /= A.hkv;
+    const int h = hk * A.group + id % A.group;
+    id /= A.group;
+    const int b = id % (A.seqs + A.zero_tail);
+    const int tile = row_tiles - 1 - id / (A.seqs + A.zero_tail);
+    if (b == A.seqs) {                                 // rows of no sequence, before the first and behind the last
+        const int a = min(max(A.cu[0], 0), A.rows), z = min(max(A.cu[A.seqs], a), A.rows);
+        const int none = a + A.rows - z;
+        for (int r = tile * ROWS + (threadIdx.x >> 5); r < none; r += 8) {
+            if (r >= tile * ROWS + ROWS && tile != row_tiles - 1) break;
+            uint16_t* o = reinterpret_cast<uint16_t*>(A.out) + ((long)(r < a ? r : z + r - a) * A.hq + h) * A.d;
+            for (int d = threadIdx.x & 31; d < A.d; d += 32) o[d] = 0;
+        }
+        return;
+    }
+    const int start = min(max(A.cu[b], 0), A.rows), end = min(max(A.cu[b + 1], start), A.rows);
+    const int len = end - start;
+    const int q0 = tile * ROWS;
+    if (q0 >= len) return;
+    const int D = A.d, chunks = D >> 3;
+    const uint16_t* kp = reinterpret_cast<const uint16_t*>(A.k) + (long)start * A.k_row + hk * A.k_head;
+    const uint16_t* vp = reinterpret_cast<const uint16_t*>(A.v) + (long)start * A.v_row + hk * A.v_head;
+
+    // this wave's rows of q
+    const int wq = q0 + 32 * wave, row = wq + n;
+    u4 q[KS];
+    {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(A.q) + (long)(start + min(row, len - 1)) * A.q_row +
+                             h * A.q_head;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int c = 2 * s + hf;
+            q[s] = c < chunks ? *reinterpret_cast<const u4*>(qp + 8 * c) : u4{0, 0, 0, 0};
+        }
+    }
+    // K steps past the head's values: zeros in both buffers
+    for (int c = chunks; c < 2 * KS; ++c)
+        for (int x = threadIdx.x; x < 2 * KT; x += 64 * WAVES)
+            *reinterpret_cast<u4*>(lds + (x / KT) * 2 * TILE + 16 * k_at<CP>(x % KT, c)) = u4{0, 0, 0, 0};
+
+    auto stage = [&](int t, int buf) {
+#pragma unroll
+        for (int i = 0; i < KT * CP / (64 * WAVES); ++i) {
+            const int pos = (i * WAVES + wave) * 64 + lane;       // chunk position in the tile
+            const int r = pos / CP, cx = pos % CP;
+            const int tok = min(t * KT + r, len - 1);
+            char* to = lds + buf * 2 * TILE + (i * WAVES + wave) * 1024;
+            const int ck = cx ^ (r & (CP - 1)), cv = cx ^ ((r & 3) << 2 & (CP - 1));
+            if (ck < chunks)
+                __builtin_amdgcn_global_load_lds((glb_ptr)(kp + (long)tok * A.k_row + 8 * ck), (lds_ptr)to, 16, 0, 0);
+            if (cv < chunks)
+                __builtin_amdgcn_global_load_lds((glb_ptr)(vp + (long)tok * A.v_row + 8 * cv), (lds_ptr)(to + TILE),
+                                                 16, 0, 0);
+        }
+    };
+
+    f16v acc[DT32];
+#pragma unroll
+    for (int i = 0; i < DT32; ++i) acc[i] = zero16();
+    float M = LOW, l = 0.f;
+    const float cc = A.scale * 1.44269504088896341f;
+
+    // V^T operand of d tile i, token step s: two transposed reads of four tokens
+    const int tr_row = 4 * hf + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const int tr_byte = 8 * (lane & 1);
+    auto v_operand = [&](const char* vt, int i, int s) {
+        union { s4 h[2]; u4 v; } o;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int r = 16 * s + 8 * p + tr_row;
+            const char* at = vt + 16 * v_at<CP>(r, 4 * i + tr_chunk) + tr_byte;
+            o.h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
+        }
+        return o.v;
+    };
+
+    bool odd_values = false;                                      // some V tile on the diagonal is not all finite
+    auto tile_step = [&](int t, auto edge_tag) {
+        constexpr bool EDGE = decltype(edge_tag)::value;          // some row does not see all of the tile
+        const char* kt = lds + (t & 1) * 2 * TILE;
+        const char* vt = kt + TILE;
+        f16v s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s[i] = zero16();
+#pragma unroll
+            for (int st = 0; st < KS; ++st)
+                s[i] = mfma<DT>(*reinterpret_cast<const u4*>(kt + 16 * k_at<CP>(32 * i + n, 2 * st + hf)), q[st], s[i]);
+        }
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int tok = t * KT + 32 * i + 8 * (j >> 2) + 4 * hf + (j & 3);
+                    s[i][j] = tok <= row ? s[i][j] : -__builtin_inff();
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * cc;
+        if (__builtin_amdgcn_ballot_w64(top > M + SLACK) != 0) {
+            const float to = top > M + SLACK ? top : M;
+            const float f = __builtin_amdgcn_exp2f(M - to);
+            M = to;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < DT32; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[i][j] *= f;
+        }
+        u4 w[4];                                                  // 16 tokens a step
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], cc, -M));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j + 1], cc, -M));
+                l += x + y;
+                w[2 * i + (j >> 3)][(j & 7) >> 1] = pack2<DT>(x, y);
+            }
+        if constexpr (EDGE) {
+            uint32_t bad = 0;
+            for (int x = lane; x < KT * CP; x += 64) {
+                const int r = x / CP, c = (x % CP) ^ ((r & 3) << 2 & (CP - 1));
+                if (c >= chunks) continue;
+                const u4 v = *reinterpret_cast<const u4*>(vt + 16 * x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= not_finite(v[e]);
+            }
+            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+                odd_values = true;
+#pragma unroll
+                for (int i = 0; i < DT32; ++i)
+#pragma unroll
+                    for (int st = 0; st < 4; ++st) {
+                        u4 v = v_operand(vt, i, st);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] &= ~not_finite(v[e]);
+                        acc[i] = mfma<DT>(v, w[st], acc[i]);
+                    }
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DT32; ++i)
+#pragma unroll
+            for (int st = 0; st < 4; ++st) acc[i] = mfma<DT>(v_operand(vt, i, st), w[st], acc[i]);
+    };
+
+    const int tiles = (min(q0 + ROWS, len) + KT - 1) / KT;       // the workgroup's last row sees up to itself
+    const int whole = (wq + 1) / KT;                              // tiles that every row of this wave sees all of
+    stage(0, 0);
+    for (int t = 0; t < tiles; ++t) {
+        __syncthreads();                                          // tile t has landed; tile t - 1 has been read
+        if (t + 1 < tiles) stage(t + 1, (t + 1) & 1);
+        if (t < whole) tile_step(t, std::integral_constant<bool, false>{});
+        else if (t * KT <= wq + 31) tile_step(t, std::integral_constant<bool, true>{});
+    }
+    l += __shfl_xor(l, 32);
+    if (row >= len) return;
+    const float inv = 1.f / l;
+    uint16_t* o = reinterpret_cast<uint16_t*>(A.out) + ((long)(start + row) * A.hq + h) * D;
+#pragma unroll
+    for (int i = 0; i < DT32; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 32 * i + 8 * j + 4 * hf;
+            if (d < D) {
+                uint2 v;
+                v.x = pack2<DT>(acc[i][4 * j] * inv, acc[i][4 * j + 1] * inv);
+                v.y = pack2<DT>(acc[i][4 * j + 2] * inv, acc[i][4 * j + 3] * inv);
+                *reinterpret_cast<uint2*>(o + d) = v;
+            }
+        }
+    if (odd_values) {                                             // what the row sees of them
+#pragma unroll 1
+        for (int tok = whole * KT; tok <= row; ++tok)
+#pragma unroll 1
+            for (int d = 4 * hf; d < D; d += (d & 3) == 3 ? 5 : 1) {
+                const uint16_t x = vp[(long)tok * A.v_row + d];
+                if (not_finite(x) != 0) store_f<DT>(o, d, load_f<DT>(o, d) + load_f<DT>(&x, 0));
+            }
+    }
+}
+
+struct Built {
+    const void* f;
+    int cp;
+};
+
+template <int DT>
+Built kernel_for(int d) {
+    switch ((d + 15) / 16) {
+        case 1: case 2: return {(const void*)prompt_attn_kernel<DT, 2, 4>, 4};
+        case 3: return {(const void*)prompt_attn_kernel<DT, 3, 8>, 8};
+        case 4: return {(const void*)prompt_attn_kernel<DT, 4, 8>, 8};
+        case 5: return {(const void*)prompt_attn_kernel<DT, 5, 16>, 16};
+        case 6: return {(const void*)prompt_attn_kernel<DT, 6, 16>, 16};
+        case 7: return {(const void*)prompt_attn_kernel<DT, 7, 16>, 16};
+        case 8: return {(const void*)prompt_attn_kernel<DT, 8, 16>, 16};
+        case 9: case 10: case 11: case 12: return {(const void*)prompt_attn_kernel<DT, 12, 32>, 32};
+        default: return {(const void*)prompt_attn_kernel<DT, 16, 32>, 32};
+    }
+}
+
+}  // namespace
+
+hipError_t launch_prompt_attn(const PromptArgs& A, int dt, hipStream_t stream) {
+    const Built k = dt == DT_F16 ? kernel_for<DT_F16>(A.d) : kernel_for<DT_BF16>(A.d);
+    PromptArgs a = A;
+    int row_tiles = (A.longest + ROWS - 1) / ROWS;
+    const int lds = 4 * KT * k.cp * 16;
+    if (hipError_t e = lds_limit_raise(k.f, lds); e != hipSuccess) return e;
+    void* args[] = {&a, &row_tiles};
+    const long grid = (long)row_tiles * (A.seqs + A.zero_tail) * A.hq;
+    return launch(k.f, dim3((unsigned)grid), dim3(64 * WAVES), args, lds, stream);
+}
+
+}  // namespace cbk

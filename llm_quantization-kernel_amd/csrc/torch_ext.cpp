@@ -441,6 +441,8 @@ void stream_probe(const Tensor& src, int64_t unroll, int64_t block, bool store, 
 
 }  // namespace
 
+void bind_attention(py::module& m);      // torch_attn.cpp
+
 PYBIND11_MODULE(_ext, m) {
     m.doc() = "crispybits_kernels op bindings over libcrispybits_hip.so (gfx950)";
     m.def("packed_gemv", &packed_gemv, "Packed W2/W3/W4 decode GEMV (streaming, split-K by plan)");
@@ -463,5 +465,6 @@ PYBIND11_MODULE(_ext, m) {
     m.def("timer_stop", &timer_stop, "Disarm the timer: (total ms, per-launch ms)");
     m.def("stream_probe", &stream_probe, "One streaming launch over a tensor's bytes (the measurement floor)",
           py::arg("src"), py::arg("unroll"), py::arg("block"), py::arg("store"), py::arg("sink"));
+    bind_attention(m);
     m.attr("ABI_VERSION") = cbk_abi_version();
 }
