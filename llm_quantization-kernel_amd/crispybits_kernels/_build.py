@@ -34,8 +34,12 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-f
              "-Wno-unused-result", "-I" + CSRC, "-I" + os.path.join(os.path.dirname(ROOT), "include")]
 
 
-# Per-file compiler flags beside HIP_FLAGS (none at present).
-FILE_FLAGS: dict = {}
+# Per-file compiler flags beside HIP_FLAGS.  The attention kernels work on their accumulators between the products:
+# with those in AGPRs (the compiler's choice for matrix instructions) each tile moved them out and back, 72 moves
+# beside 190 other vector instructions a block of kv4_attn.
+FILE_FLAGS: dict = {"kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                    "prompt_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                    "prompt_attn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _hipcc() -> str:

@@ -91,7 +91,7 @@ AttnPlan plan_attn(int64_t seqs, int64_t t, int64_t heads, int64_t kv_heads, int
     p.cols = (int)std::min<int64_t>(p.rows, 16);
     const int64_t units = std::max<int64_t>(1, seqs * kv_heads * p.tiles);
     const int64_t blocks = width * (page / KV4_BLOCK);
-    p.splits = std::max<int64_t>(1, std::min((FILL + units - 1) / units, blocks / MIN_BLOCKS));
+    p.splits = std::max<int64_t>(1, std::min({(FILL + units - 1) / units, blocks / MIN_BLOCKS, (int64_t)KV4_MAX_SPLITS}));
     p.floats = p.splits > 1 ? units * p.splits * p.cols * (d + 2) : 0;
     return p;
 }

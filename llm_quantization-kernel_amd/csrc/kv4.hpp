@@ -29,6 +29,7 @@ namespace cbk {
 
 constexpr int KV4_BLOCK = 32;                        // tokens of a block
 constexpr int KV4_MAX_D = 256;
+constexpr int KV4_MAX_SPLITS = 256;                   // workgroups that share a sequence in attention
 // the smallest scale a token may have: values below it count as zeros
 constexpr float KV4_MIN_SCALE = 0x1p-100f;
 
@@ -94,7 +95,7 @@ struct Kv4AttnArgs {
     Kv4View c;
     const void* q;             // [seqs, t, hq, d] contiguous, 16-byte aligned
     void* out;                 // the same
-    float* partial;            // [seqs, heads, row tiles, splits, cols (d + 2)] when splits > 1
+    float* partial;            // [seqs, heads, row tiles, splits, cols, d], then [..., cols, 2]: splits > 1
     uint32_t* split_cnt;       // arrival counter per (seq, head, row tile); nullptr: a combine launch
     int t, hq, group;          // new tokens a sequence, query heads, query heads per kv head
     int rows, tiles, cols;     // t * group query rows per kv head, tiles of 16 of them, rows of a partial
