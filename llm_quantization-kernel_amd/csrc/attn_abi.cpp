@@ -74,25 +74,29 @@ int check_rows(const char* what, int64_t rows, const int32_t* cu, int64_t seqs) 
     return CBK_OK;
 }
 
-// Workgroups that a sequence's blocks of 32 tokens may go to: enough for FILL of them over the chip (four on each of
-// 256 CUs), each with at least a block a wave.
-constexpr int64_t FILL = 1024;
-constexpr int MIN_BLOCKS = 4;
+// Workgroups of a cache attention call: as many as are on the chip's 256 CUs at once, and where the work is
+// less, one for each unit or MIN_BLOCKS blocks.  Units cannot be cut where none has more than KV4_WHOLE blocks.
+constexpr int64_t CUS = 256;
+static_assert(3 * CUS <= SPLIT_COUNTERS, "a counter per workgroup");
+constexpr int MIN_BLOCKS = 12;
+constexpr int UNIT_COST = 12;
 
 struct AttnPlan {
-    int64_t rows, tiles, splits, floats;
+    int64_t rows, tiles, groups, floats, blocks;
     int cols;
 };
 
-AttnPlan plan_attn(int64_t seqs, int64_t t, int64_t heads, int64_t kv_heads, int d, int64_t page, int64_t width) {
+AttnPlan plan_attn(int dtype, int64_t seqs, int64_t t, int64_t heads, int64_t kv_heads, int d, int64_t page,
+                   int64_t width) {
     AttnPlan p;
     p.rows = t * (heads / kv_heads);
     p.tiles = (p.rows + 15) / 16;
     p.cols = (int)std::min<int64_t>(p.rows, 16);
     const int64_t units = std::max<int64_t>(1, seqs * kv_heads * p.tiles);
-    const int64_t blocks = width * (page / KV4_BLOCK);
-    p.splits = std::max<int64_t>(1, std::min({(FILL + units - 1) / units, blocks / MIN_BLOCKS, (int64_t)KV4_MAX_SPLITS}));
-    p.floats = p.splits > 1 ? units * p.splits * p.cols * (d + 2) : 0;
+    const int64_t most = std::max<int64_t>(1, width * (page / KV4_BLOCK));
+    p.blocks = units * (most + UNIT_COST);
+    p.groups = std::min(kv4_waves(kv4_ns(d), dtype) * CUS, std::max(units, p.blocks / MIN_BLOCKS));
+    p.floats = most > KV4_WHOLE && p.groups > 1 ? 2 * p.groups * p.cols * (d + 2) : 0;
     return p;
 }
 
@@ -160,7 +164,7 @@ int64_t cbk_kv4_attention_partial_floats(int64_t num_seqs, int64_t t, int64_t he
     if (num_seqs <= 0 || t <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 ||
         cbk_kv4_page_words(head_dim, page_size) < 0 || table_width < 0)
         return 0;
-    return plan_attn(num_seqs, t, heads, kv_heads, head_dim, page_size, table_width).floats;
+    return plan_attn(CBK_F16, num_seqs, t, heads, kv_heads, head_dim, page_size, table_width).floats;      // the most of any type
 }
 
 int cbk_kv4_attention(const void* q, int dtype, int64_t num_seqs, int64_t t, int64_t heads,
@@ -178,21 +182,22 @@ int cbk_kv4_attention(const void* q, int dtype, int64_t num_seqs, int64_t t, int
     if (num_seqs == 0 || t == 0) return CBK_OK;
     if (!q || !out) return fail(CBK_EINVAL, "%s: q and out must be non-null", what);
     if (!aligned(q) || !aligned(out)) return fail(CBK_EINVAL, "%s: q and out must be 16-byte aligned", what);
-    const AttnPlan p = plan_attn(num_seqs, t, heads, kv_heads, head_dim, page_size, table_width);
+    const AttnPlan p = plan_attn(dtype, num_seqs, t, heads, kv_heads, head_dim, page_size, table_width);
     if (kv_heads * p.tiles > MOST_GRID) return fail(CBK_EINVAL, "%s: too many new tokens", what);
+    if (p.blocks > INT32_MAX / 2) return fail(CBK_EINVAL, "%s: block table too wide for the call's sequences and heads", what);
     if (p.floats > 0 && (!partial || partial_floats < p.floats))
         return fail(CBK_EINVAL, "%s: partial must hold %lld floats", what, (long long)p.floats);
     A.q = q, A.out = out;
     A.partial = p.floats > 0 ? partial : nullptr;
     A.t = (int)t, A.hq = (int)heads, A.group = (int)(heads / kv_heads);
     A.rows = (int)p.rows, A.tiles = (int)p.tiles, A.cols = p.cols;
-    A.splits = (int)p.splits, A.min_blocks = MIN_BLOCKS;
+    A.groups = (int)p.groups, A.min_blocks = MIN_BLOCKS, A.unit_cost = UNIT_COST;
     A.scale = scale;
     A.div_group = make_fastdiv((uint32_t)A.group);
     DeviceGuard guard(device);
     if (guard.err != hipSuccess) return hip_fail(guard.err, "set device");
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    A.split_cnt = p.splits > 1 && num_seqs * kv_heads * p.tiles <= SPLIT_COUNTERS ? attn_window(device, s) : nullptr;
+    A.split_cnt = p.floats > 0 ? attn_window(device, s) : nullptr;
     const hipError_t e = launch_kv4_attn(A, dtype, s);
     return e == hipSuccess ? CBK_OK : hip_fail(e, what);
 }

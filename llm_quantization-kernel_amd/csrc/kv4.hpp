@@ -29,7 +29,7 @@ namespace cbk {
 
 constexpr int KV4_BLOCK = 32;                        // tokens of a block
 constexpr int KV4_MAX_D = 256;
-constexpr int KV4_MAX_SPLITS = 256;                   // workgroups that share a sequence in attention
+constexpr int KV4_WHOLE = 8;                           // attention does not cut units of this many blocks
 // the smallest scale a token may have: values below it count as zeros
 constexpr float KV4_MIN_SCALE = 0x1p-100f;
 
@@ -59,12 +59,18 @@ struct Kv4View {
     int width, seqs;
 };
 
+// An entry of an index tensor that no kernel of the call writes, read at a wave-uniform place: through the constant
+// address space, so that it is a scalar load, which waits for no vector load under way.
+__device__ __forceinline__ int index_at(const int32_t* p, long i) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
 // The first word of block `blk` of sequence `b`, head `h`; nullptr where the table has no page of the
 // pool for it (behind the table, or an entry outside the pool): such tokens do not exist.
 __device__ __forceinline__ uint32_t* kv4_block(const Kv4View& C, int b, int blk, int h) {
     const int p = blk >> C.page_shift;
     if (blk < 0 || p >= C.width) return nullptr;
-    const int page = C.table[(long)b * C.width + p];
+    const int page = index_at(C.table, (long)b * C.width + p);
     if ((unsigned)page >= (unsigned)C.num_pages) return nullptr;
     const long row = ((long)page * C.heads + h) << C.page_shift;
     return C.pages + (row + (blk & ((1 << C.page_shift) - 1))) * kv4_block_words(C.ns);
@@ -91,15 +97,18 @@ hipError_t launch_kv4_append(const Kv4StoreArgs& A, int dt, hipStream_t stream);
 hipError_t launch_kv4_read(const Kv4StoreArgs& A, int dt, hipStream_t stream);
 
 // kv4_attn.hip
+// Workgroups of the attention kernel that a CU holds: by its registers (up to 128 values three, fp32 at 128 and more two).
+__host__ __device__ constexpr int kv4_waves(int ns, int dt) { return ns < 4 || (ns == 4 && dt != DT_F32) ? 3 : 2; }
 struct Kv4AttnArgs {
     Kv4View c;
     const void* q;             // [seqs, t, hq, d] contiguous, 16-byte aligned
     void* out;                 // the same
-    float* partial;            // [seqs, heads, row tiles, splits, cols, d], then [..., cols, 2]: splits > 1
-    uint32_t* split_cnt;       // arrival counter per (seq, head, row tile); nullptr: a combine launch
+    float* partial;            // [2 groups][cols, d], then [2 groups][cols, 2]; nullptr: no unit can be cut
+    uint32_t* split_cnt;       // an arrival counter per workgroup; nullptr: a combine launch
     int t, hq, group;          // new tokens a sequence, query heads, query heads per kv head
     int rows, tiles, cols;     // t * group query rows per kv head, tiles of 16 of them, rows of a partial
-    int splits, min_blocks;    // workgroups a sequence's blocks go to at most; blocks each takes at least
+    int groups, min_blocks;    // workgroups; blocks each takes at least where units are cut
+    int unit_cost;             // blocks that a unit costs beside its own
     float scale;
     FastDiv div_group;
 };

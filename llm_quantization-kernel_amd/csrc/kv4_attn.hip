@@ -18,9 +18,13 @@
 // below the largest still count; the sum of p is held with the same factor.  M moves only when it would
 // have to by 3 or more (the accumulators are rescaled then).
 //
-// A sequence's blocks go to `splits` workgroups of four waves at most (min_blocks each at least; counted
-// from the length on the device), whose waves take them in turn, the next block's loads under way; waves meet in LDS, workgroups through fp32 partials
-// and an arrival counter (or a second launch), in a fixed order.
+// Work: a unit is a sequence, kv head and tile of 16 query rows, of as many blocks as the sequence has (one at
+// least, whose workgroup writes the zeros of an empty one).  The blocks of all units stand in one row, sequence by
+// sequence, and each workgroup takes an equal piece of it, counted from the lengths on the device: ragged batches
+// and single long sequences load the chip alike.  Its four waves take a unit's blocks in turn, the next block's
+// loads under way, and meet in LDS.  A unit cut by a border is joined from fp32 partials, at most two a
+// workgroup, by the last of its workgroups to arrive (or a second launch), in a fixed order.  Units of few blocks are not
+// cut: the workgroup that has their first block takes them whole.
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
 
@@ -84,7 +88,7 @@ __device__ __forceinline__ float group_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// One block's words as a lane holds them.
+// One block's words as a lane holds them, keys and values loaded apart.
 template <int NS, bool EXACT>
 struct Block {
     uint32_t k[2][NS];
@@ -92,17 +96,25 @@ struct Block {
     u4 km[2], vm[2];
     uint32_t kz[2];                    // EXACT: the words of the tokens whose codes this lane decodes
 
-    __device__ __forceinline__ void load(const uint32_t* p, int lane) {
+    // byte offsets from the (uniform) block, 32-bit: one register an address
+    __device__ __forceinline__ void load_k(const uint32_t* p, uint32_t lane) {
+        const char* base = reinterpret_cast<const char*>(p);
+        const uint32_t ko = ((lane & 15) * 4 * NS + (lane >> 4) * NS) * 4, mo = 1024 * NS + (lane >> 4) * 16;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            __builtin_memcpy(k[i], base + (ko + i * 256 * NS), 4 * NS);
+            km[i] = *reinterpret_cast<const u4*>(base + (mo + 64 * i));
+            if constexpr (EXACT) kz[i] = *reinterpret_cast<const uint32_t*>(base + (1024 * NS + 64 * i + (lane & 15) * 4));
+        }
+    }
+    __device__ __forceinline__ void load_v(const uint32_t* p, uint32_t lane) {
         constexpr int PW = kv4_piece(NS);
-        const uint32_t* kp = p + (lane & 15) * 4 * NS + (lane >> 4) * NS;
+        const char* base = reinterpret_cast<const char*>(p);
+        const uint32_t vo = 512 * NS + lane * PW * 4, mo = 1024 * NS + 128 + (lane >> 4) * 16;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) __builtin_memcpy(k[i], kp + i * 64 * NS, 4 * NS);
-        const uint32_t* vp = p + 128 * NS + lane * PW;
+        for (int i = 0; i < 2; ++i) vm[i] = *reinterpret_cast<const u4*>(base + (mo + 64 * i));
 #pragma unroll
-        for (int i = 0; i < 2 * NS / PW; ++i) __builtin_memcpy(v + i * PW, vp + i * 64 * PW, 4 * PW);
-        const u4* mp = reinterpret_cast<const u4*>(p + 256 * NS) + (lane >> 4);
-        km[0] = mp[0], km[1] = mp[4], vm[0] = mp[8], vm[1] = mp[12];
-        if constexpr (EXACT) kz[0] = p[256 * NS + (lane & 15)], kz[1] = p[256 * NS + 16 + (lane & 15)];
+        for (int i = 0; i < 2 * NS / PW; ++i) __builtin_memcpy(v + i * PW, base + (vo + i * 256 * PW), 4 * PW);
     }
 };
 
@@ -115,27 +127,98 @@ __device__ __forceinline__ void load8(const void* p, long i, float (&x)[8]) {
     for (int j = 0; j < 8; ++j) x[j] = Dt<DT>::to_f(v.v[j]);
 }
 
-// Workgroups that share sequence b's blocks, and the blocks each takes.
-__device__ __forceinline__ void shares(const Kv4AttnArgs& A, int len, int& blocks, int& per, int& active) {
-    const int room = min((long)A.c.width << A.c.page_shift, (long)1 << 26);
-    blocks = min((max(len, 0) + 31) >> 5, room);
-    per = max((blocks + A.splits - 1) / A.splits, A.min_blocks);
-    active = max((blocks + per - 1) / per, 1);
+// Blocks of a sequence in the row of all units' blocks.
+__device__ __forceinline__ int blocks_of(const Kv4AttnArgs& A, int len) {
+    const int room = A.c.width << A.c.page_shift;
+    return max(min((max(len, 0) + 31) >> 5, room), 1);
 }
 
-// The partials of a (sequence, head, row tile) and split: [cols][D] sums, and behind those of all units
-// [cols][2], each row's reference M and sum of p.  They pass between workgroups on any XCD: written and read
-// past the L2s (sc1), as split_arrive's note says.
+// Sum over lanes 0 .. lane.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);      // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+// The row of blocks and this workgroup's piece of it: positions count blocks, a sequence's units (kv heads x row
+// tiles) follow each other.  A unit costs more than its blocks (its query, the waves' meeting): it stands
+// for unit_cost blocks more, before its own.
+struct Row {
+    int len0;                          // this lane's length among the first 64 sequences
+    int total, piece, whole;           // blocks; of a piece; units of at most so many are not cut
+
+    __device__ __forceinline__ int count(const Kv4AttnArgs& A, int b0, int lane) const {
+        const int b = b0 + lane;
+        return b < A.c.seqs ? blocks_of(A, b0 == 0 ? len0 : A.c.lens[b]) + A.unit_cost : 0;
+    }
+    __device__ __forceinline__ void set(const Kv4AttnArgs& A, int lane) {
+        len0 = lane < A.c.seqs ? A.c.lens[lane] : 0;
+        int sum = 0;
+        uint64_t large = 0;
+        for (int b0 = 0; b0 < A.c.seqs; b0 += 64) {
+            const int c = count(A, b0, lane);
+            large |= __builtin_amdgcn_ballot_w64(c > KV4_WHOLE + A.unit_cost);
+            sum += __builtin_amdgcn_readlane(wave_scan(c), 63);
+        }
+        total = sum * A.c.heads * A.tiles;
+        piece = max((total + A.groups - 1) / A.groups, large ? A.min_blocks : 1);
+        whole = max(KV4_WHOLE, piece >> 3);
+    }
+};
+
+// A unit: its sequence, which of the sequence's units, its blocks and the first one's position.
+struct Unit {
+    int b, j, blocks, start;
+};
+
+__device__ __forceinline__ Unit unit_at(const Kv4AttnArgs& A, const Row& R, int x, int lane) {
+    const int each = A.c.heads * A.tiles;
+    Unit u;
+    int before = 0;
+    for (int b0 = 0;; b0 += 64) {
+        const int c = R.count(A, b0, lane), upto = wave_scan(c);
+        const uint64_t m = __builtin_amdgcn_ballot_w64(b0 + lane < A.c.seqs && (before + upto) * each <= x);
+        const int k = __builtin_popcountll(m);
+        if (k < 64 || b0 + 64 >= A.c.seqs) {
+            const int i = min(k, 63);
+            u.b = b0 + i;
+            u.blocks = __builtin_amdgcn_readlane(c, i);
+            const int first = (before + __builtin_amdgcn_readlane(upto, i) - u.blocks) * each;
+            u.j = (x - first) / max(u.blocks, 1);
+            u.start = first + u.j * u.blocks + A.unit_cost;
+            u.blocks -= A.unit_cost;
+            return u;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+
+// The partials of a slot (two a workgroup: its piece's first unit, and a later one): [cols][D] sums, and behind
+// those of all slots [cols][2], each row's reference M and sum of p.  They pass between workgroups on any XCD: written
+// and read past the L2s (sc1), as split_arrive's note says.
 constexpr int SC1 = 16;
-__device__ __forceinline__ long part_sums(const Kv4AttnArgs& A, int unit, int split) {
-    return ((long)unit * A.splits + split) * A.cols * A.c.d;
+__device__ __forceinline__ float* part_sums(const Kv4AttnArgs& A, int slot) {
+    return A.partial + (long)slot * A.cols * A.c.d;
 }
-__device__ __forceinline__ float* part_rows(const Kv4AttnArgs& A, int unit, int split) {
-    const long units = (long)A.c.seqs * A.c.heads * A.tiles;
-    return A.partial + units * A.splits * A.cols * A.c.d + ((long)unit * A.splits + split) * A.cols * 2;
+__device__ __forceinline__ float* part_rows(const Kv4AttnArgs& A, int slot) {
+    return A.partial + 2l * A.groups * A.cols * A.c.d + (long)slot * A.cols * 2;
 }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float* p, long floats) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, (int)min(floats * 4, (long)0x7FFFFFF0), 0x00027000);
+// The parts of a unit that borders cut: workgroups first .. first + count - 1; its part in the first is that one's
+// later slot unless the unit starts its piece.
+struct Parts {
+    int first, count, later;
+    __device__ __forceinline__ int slot(int i) const { return 2 * (first + i) + (i == 0 ? later : 0); }
+};
+__device__ __forceinline__ Parts parts_of(const Row& R, const Unit& u) {
+    Parts p;
+    p.first = u.start / R.piece;
+    p.count = (u.start + u.blocks - 1) / R.piece - p.first + 1;
+    p.later = u.start != p.first * R.piece ? 1 : 0;
+    return p;
 }
 
 template <int DT>
@@ -144,77 +227,111 @@ __device__ __forceinline__ long out_at(const Kv4AttnArgs& A, int b, int h, int r
     return (((long)b * A.t + i) * A.hq + h * A.group + (row - i * A.group)) * A.c.d;
 }
 
-// LDS of the combine: what each split's row counts for, and the sums of the thread groups.
+// LDS of the combine: what each part's row counts for, and the sums of the thread groups.
+constexpr int SHARES = 64;             // parts whose shares are held at once
 struct CombineLds {
-    float share[KV4_MAX_SPLITS * 16];
+    float share[SHARES * 16];
     float m[16][16], l[16][16];
     float4 sum[64 * WAVES];
 };
 
-// Adds the active workgroups' partials of a unit, in order, and writes its rows.  Threads share the splits: all
-// loads of a thread are independent.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float* p, long floats) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, (int)min(floats * 4, (long)0x7FFFFFF0), 0x00027000);
+}
+
+// Adds a cut unit's partials in order and writes its rows.  Threads share the parts.  Up to 64 parts (8 a thread of
+// the sums) all loads are under way before the first is waited for: the joining workgroup is the call's last one, and
+// its latencies add up.
 template <int DT>
-__device__ __forceinline__ void combine(const Kv4AttnArgs& A, CombineLds& L, int unit, int b, int h, int tile, int active) {
+__device__ __forceinline__ void combine(const Kv4AttnArgs& A, CombineLds& L, const Parts& P, int b, int h, int tile) {
+    constexpr int EARLY = 8;
     const int D = A.c.d, cols = min(A.cols, A.rows - 16 * tile), tid = threadIdx.x;
-    {
-        const int c = tid & 15, s0 = tid >> 4;
-        const float* r = part_rows(A, unit, 0) + 2 * c;
-        float m = LOW, l = 0.f;
-        if (c < cols)
-            for (int s = s0; s < active; s += 16) m = fmaxf(m, partial_get(r + (long)s * A.cols * 2));
-        L.m[s0][c] = m;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, L.m[i][c]);
-        if (c < cols)
-            for (int s = s0; s < active; s += 16) {
-                const float* q = r + (long)s * A.cols * 2;
-                const float f = __builtin_amdgcn_exp2f(partial_get(q) - m);
-                L.share[s * cols + c] = f;
-                l += f * partial_get(q + 1);
-            }
-        L.l[s0][c] = l;
-        __syncthreads();
-    }
+    const int col = tid & 15, s0 = tid >> 4;
+    const __amdgpu_buffer_rsrc_t sums = buffer_of(part_sums(A, 2 * P.first), 2l * P.count * A.cols * D);
+    const __amdgpu_buffer_rsrc_t rows = buffer_of(part_rows(A, 2 * P.first), 4l * P.count * A.cols);
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    // (M, sum of p) of this thread's row in part s; past the last part, or a row that is not there: nothing seen
+    auto row_of = [&](int s) {
+        const int at = s < P.count && col < cols ? ((P.slot(s) - 2 * P.first) * A.cols + col) * 8 : -1;
+        const u2 v = __builtin_amdgcn_raw_buffer_load_b64(rows, at, 0, SC1);
+        return at < 0 ? u2{__float_as_uint(LOW), 0u} : v;
+    };
     const int items = cols * (D >> 2), stride = A.cols * D * 4;
-    const int groups = max(1, 64 * WAVES / items);               // thread groups that share the splits
-    const __amdgpu_buffer_rsrc_t buf = buffer_of(A.partial + part_sums(A, unit, 0), (long)active * A.cols * D);
-    for (int x0 = 0; x0 < items; x0 += 64 * WAVES) {
-        const int grp = groups > 1 ? tid / items : 0, x = groups > 1 ? tid - grp * items : x0 + tid;
-        const int c = x / (D >> 2), d = (x - c * (D >> 2)) * 4;
-        float4 o = {0.f, 0.f, 0.f, 0.f};
-        if (x < items && grp < groups) {
-            const int at = (c * D + d) * 4;
-#pragma unroll 8
-            for (int s = grp; s < active; s += groups) {
-                const u4 v = __builtin_amdgcn_raw_buffer_load_b128(buf, at + s * stride, 0, SC1);
-                const float f = L.share[s * cols + c];
-                o.x += f * __uint_as_float(v[0]), o.y += f * __uint_as_float(v[1]);
-                o.z += f * __uint_as_float(v[2]), o.w += f * __uint_as_float(v[3]);
-            }
-        }
-        if (groups > 1) {
-            L.sum[tid] = o;
-            __syncthreads();
-            if (grp != 0) return;
-            for (int g = 1; g < groups; ++g) {
-                const float4 v = L.sum[g * items + x];
-                o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-            }
-        }
-        if (x >= items) continue;
-        float l = 0.f;
+    const int groups = max(1, 64 * WAVES / items);               // thread groups that share the parts
+    const int grp = groups > 1 ? tid / items : 0;
+    auto sum_of = [&](int s, int c, int d) {
+        const int at = s < P.count ? (P.slot(s) - 2 * P.first) * stride + (c * D + d) * 4 : -1;
+        return __builtin_amdgcn_raw_buffer_load_b128(sums, at, 0, SC1);      // past the buffer: zeros
+    };
+    u2 ml[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) l += L.l[i][c];
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const long at = out_at<DT>(A, b, h, 16 * tile + c) + d;
-        store_f<DT>(A.out, at, o.x * inv), store_f<DT>(A.out, at + 1, o.y * inv);
-        store_f<DT>(A.out, at + 2, o.z * inv), store_f<DT>(A.out, at + 3, o.w * inv);
+    for (int i = 0; i < 4; ++i) ml[i] = row_of(s0 + 16 * i);
+    u4 early[EARLY];
+    {
+        const int x = groups > 1 ? tid - grp * items : tid, c = min(x / (D >> 2), cols - 1), d = (x - x / (D >> 2) * (D >> 2)) * 4;
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i) early[i] = sum_of(grp < groups ? grp + i * groups : P.count, c, d);
+    }
+    float m = LOW, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, __uint_as_float(ml[i][0]));
+    for (int s = s0 + SHARES; s < P.count; s += 16) m = fmaxf(m, __uint_as_float(row_of(s)[0]));
+    L.m[s0][col] = m;
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, L.m[i][col]);
+    for (int x0 = 0; x0 < items; x0 += 64 * WAVES) {
+        const int x = groups > 1 ? tid - grp * items : x0 + tid;
+        const int c = min(x / (D >> 2), cols - 1), d = (x - x / (D >> 2) * (D >> 2)) * 4;
+        float4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < P.count; p0 += SHARES) {
+            const int p1 = min(p0 + SHARES, P.count);
+            if (x0 == 0 || P.count > SHARES) {                   // the shares of parts p0 .. p1
+                lds_barrier();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const u2 v = p0 == 0 ? ml[i] : row_of(p0 + s0 + 16 * i);
+                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(v[0]) - m);
+                    if (col < cols) L.share[(s0 + 16 * i) * 16 + col] = f;
+                    if (x0 == 0) l += f * __uint_as_float(v[1]);
+                }
+                lds_barrier();
+            }
+            if (x < items && grp < groups) {
+                for (int s = p0 + grp; s < p1;) {
+                    if (x0 != 0 || s != grp) {                   // the next batch
+#pragma unroll
+                        for (int i = 0; i < EARLY; ++i) early[i] = sum_of(s + i * groups, c, d);
+                    }
+#pragma unroll
+                    for (int i = 0; i < EARLY; ++i, s += groups) {
+                        const float f = s < p1 ? L.share[(s - p0) * 16 + c] : 0.f;
+                        o.x += f * __uint_as_float(early[i][0]), o.y += f * __uint_as_float(early[i][1]);
+                        o.z += f * __uint_as_float(early[i][2]), o.w += f * __uint_as_float(early[i][3]);
+                    }
+                }
+            }
+        }
+        if (x0 == 0) L.l[s0][col] = l;
+        if (groups > 1) L.sum[tid] = o;
+        lds_barrier();
+        if (grp > 0 || x >= items) continue;
+        for (int g = 1; g < groups; ++g) {
+            const float4 v = L.sum[g * items + x];
+            o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        }
+        float all = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) all += L.l[i][c];
+        const float inv = all == 0.f ? 0.f : 1.f / all;
+        const long to = out_at<DT>(A, b, h, 16 * tile + c) + d;
+        store_f<DT>(A.out, to, o.x * inv), store_f<DT>(A.out, to + 1, o.y * inv);
+        store_f<DT>(A.out, to + 2, o.z * inv), store_f<DT>(A.out, to + 3, o.w * inv);
     }
 }
 
 template <int NS, int DT>
-__global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
+__global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv4_attn_kernel(Kv4AttnArgs A) {
     constexpr int TILES = 2 * NS, DP = 32 * NS;
     constexpr bool EXACT = DT == DT_F32;
     constexpr int TERMS = EXACT ? 2 : 1;
@@ -231,13 +348,40 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const Kv4View& C = A.c;
-    const int split = blockIdx.x, tile = blockIdx.y / C.heads, h = blockIdx.y - tile * C.heads, b = blockIdx.z;
-    const int len = C.lens[b];
-    int blocks, per, active;
-    shares(A, len, blocks, per, active);
-    if (split >= active) return;
-    const int first = split * per, last = min(first + per, blocks);
     const int D = C.d;
+    const int group = blockIdx.x;
+    Row R;
+    R.set(A, lane);
+    int x = group * R.piece;
+    const int end = min(x + R.piece, R.total);
+    for (; x < end; __syncthreads()) {
+    const Unit U = unit_at(A, R, x, lane);
+    const bool small = U.blocks <= R.whole;
+    const int from = max(x - U.start, 0), upto = small ? U.blocks : min(U.blocks, end - U.start);
+    // a small unit that starts before the piece is another workgroup's, and so is one whose blocks start behind it
+    const bool mine = small ? x == U.start - A.unit_cost : upto > 0;
+    x = U.start + max(upto, 0);
+    if (!mine) continue;
+    const int part_slot = 2 * group + (from == 0 && U.start != group * R.piece ? 1 : 0);
+    const int b = U.b, h = U.j / A.tiles, tile = U.j - h * A.tiles;
+    const int len = index_at(C.lens, b);
+    const int first = from, last = len > 0 && C.num_pages > 0 ? upto : 0;
+
+    // The wave's blocks in turn.  A block without a page counts as unseen; its loads (and those past the last block) go
+    // to the pool's first block, so that the loads under way are always as many and a step waits for its own alone.
+    Block<NS, EXACT> B;
+    auto where = [&](int blk, bool& there) {
+        const uint32_t* p = blk < last ? kv4_block(C, b, blk, h) : nullptr;
+        there = p != nullptr;
+        return there ? p : C.pages;
+    };
+    int blk = first + wave;
+    bool there = false;
+    if (blk < last) {
+        const uint32_t* p = where(blk, there);
+        B.load_k(p, lane);
+        B.load_v(p, lane);
+    }
 
     // this lane's query row; its newest visible token
     const int row = 16 * tile + n;
@@ -252,14 +396,18 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
     {
         float x[NS][8];
         float top = 0.f;
+        // loads of a row and values that exist, whatever the lane's own, so that all go out at once
+        const long at = out_at<DT>(A, b, h, min(row, A.rows - 1));
+#pragma unroll
+        for (int s = 0; s < NS; ++s) load8<DT>(A.q, at + min(8 * (g * NS + s), D - 8), x[s]);
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const int d = 8 * (g * NS + s);
+            const bool has = real && 8 * (g * NS + s) < D;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[s][j] = 0.f;
-            if (real && d < D) load8<DT>(A.q, out_at<DT>(A, b, h, row) + d, x[s]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, __builtin_fabsf(x[s][j]));
+            for (int j = 0; j < 8; ++j) {
+                x[s][j] = has ? x[s][j] : 0.f;
+                top = fmaxf(top, __builtin_fabsf(x[s][j]));
+            }
         }
         top = group_max(top);
         const int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;   // top < 2^e
@@ -288,7 +436,9 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
     for (int i = 0; i < TILES; ++i) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
     float M = LOW, la = 0.f, lb = 0.f;
 
-    auto step = [&](const Block<NS, EXACT>& B, int blk) {
+    while (blk < last) {
+        bool next_there;
+        const uint32_t* next = where(blk + WAVES, next_there);
         // scores of 8 tokens: y = s (dot - z sum q), and log2 of the probability's factor = cc y
         float y[8], sv[8];
 #pragma unroll
@@ -311,11 +461,16 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
             for (int j = 0; j < 4; ++j) {
                 const uint32_t w = B.km[i][j];
                 y[4 * i + j] = __uint_as_float(w) * (EXACT ? s[j] : __builtin_fmaf(-(float)(w & 15u), qsum, s[j]));
-                sv[4 * i + j] = __uint_as_float(B.vm[i][j]);
             }
         }
-        const int base = 32 * blk + 4 * g;
-        if (32 * blk + 31 > all_see) {
+        // the next block's keys, under way from here on (kept behind the last use of this one's, in its registers)
+        __builtin_amdgcn_sched_barrier(0);
+        B.load_k(next, lane);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sv[j] = __uint_as_float(B.vm[j >> 2][j & 3]);
+        if (!there || 32 * blk + 31 > all_see) {
+            const int base = there ? 32 * blk + 4 * g : INT32_MAX / 2;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const bool seen = base + (j & 3) + 16 * (j >> 2) <= newest;
@@ -382,27 +537,10 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
 #pragma unroll
             for (int i = 0; i < TILES; ++i) acc[i] = mfma(decode(B.v[i]), wo[0].v, acc[i]);
         }
-    };
-
-    // the wave's blocks in turn, two sets of registers; a block without a page is left out
-    {
-        Block<NS, EXACT> one, two;
-        auto fetch = [&](Block<NS, EXACT>& B, int blk) {
-            const uint32_t* p = blk < last ? kv4_block(C, b, blk, h) : nullptr;
-            if (p) B.load(p, lane);
-            return p != nullptr;
-        };
-        int blk = first + wave;
-        bool has_one = fetch(one, blk), has_two;
-        while (blk < last) {
-            has_two = fetch(two, blk + WAVES);
-            if (has_one) step(one, blk);
-            blk += WAVES;
-            if (blk >= last) break;
-            has_one = fetch(one, blk + WAVES);
-            if (has_two) step(two, blk);
-            blk += WAVES;
-        }
+        __builtin_amdgcn_sched_barrier(0);
+        B.load_v(next, lane);
+        blk += WAVES;
+        there = next_there;
     }
 
     // the waves' rows meet
@@ -427,10 +565,10 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
         }
         __syncthreads();
     }
-    const int unit = (b * C.heads + h) * A.tiles + tile;
+    const bool all = from == 0 && upto == U.blocks;
     const int cols = min(16, A.rows - 16 * tile);
-    for (int x = threadIdx.x; x < cols * (D >> 2); x += 64 * WAVES) {
-        const int c = x / (D >> 2), d = (x - c * (D >> 2)) * 4;
+    for (int y = threadIdx.x; y < cols * (D >> 2); y += 64 * WAVES) {
+        const int c = y / (D >> 2), d = (y - c * (D >> 2)) * 4;
         float o[4], ls = 0.f, mt = red_m[0][c];
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) mt = fmaxf(mt, red_m[w][c]);
@@ -438,33 +576,41 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs A) {
         for (int w = 0; w < WAVES; ++w) ls += red_l[w][c] * __builtin_amdgcn_exp2f(red_m[w][c] - mt);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = red[0][c][d + i] + red[1][c][d + i];
-        if (active == 1) {
+        if (all) {
             const float inv = ls == 0.f ? 0.f : 1.f / ls;
             const long at = out_at<DT>(A, b, h, 16 * tile + c) + d;
 #pragma unroll
             for (int i = 0; i < 4; ++i) store_f<DT>(A.out, at + i, o[i] * inv);
         } else {
-            const __amdgpu_buffer_rsrc_t buf = buffer_of(A.partial + part_sums(A, unit, split), (long)A.cols * D);
+            const __amdgpu_buffer_rsrc_t buf = buffer_of(part_sums(A, part_slot), (long)A.cols * D);
             const u4 v = {__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])};
             __builtin_amdgcn_raw_buffer_store_b128(v, buf, (c * D + d) * 4, 0, SC1);
             if (d == 0) {
-                float* r = part_rows(A, unit, split) + 2 * c;
+                float* r = part_rows(A, part_slot) + 2 * c;
                 partial_put(r, mt), partial_put(r + 1, ls);
             }
         }
     }
-    if (active == 1 || !A.split_cnt) return;
-    if (split_arrive(A.split_cnt + unit, active, &flag)) combine<DT>(A, lds.combine, unit, b, h, tile, active);
+    if (all || !A.split_cnt) continue;
+    const Parts P = parts_of(R, U);
+    if (split_arrive(A.split_cnt + P.first, P.count, &flag)) combine<DT>(A, lds.combine, P, b, h, tile);
+    }
 }
 
-// The combine as a launch of its own, for calls without counters.
+// The combine as a launch of its own, for calls without counters: a workgroup joins the unit that the end of its
+// piece cuts, if its first part is there.
 template <int DT>
 __global__ __launch_bounds__(64 * WAVES) void kv4_combine_kernel(Kv4AttnArgs A) {
     __shared__ __align__(16) CombineLds lds;
-    const int tile = blockIdx.y / A.c.heads, h = blockIdx.y - tile * A.c.heads, b = blockIdx.z;
-    int blocks, per, active;
-    shares(A, A.c.lens[b], blocks, per, active);
-    if (active > 1) combine<DT>(A, lds, (b * A.c.heads + h) * A.tiles + tile, b, h, tile, active);
+    const int lane = threadIdx.x & 63, group = blockIdx.x;
+    Row R;
+    R.set(A, lane);
+    const int end = (group + 1) * R.piece;
+    if (end >= R.total) return;
+    const Unit U = unit_at(A, R, end - 1, lane);
+    if (U.blocks <= R.whole || U.start + U.blocks <= end || U.start >= end || U.start < group * R.piece) return;
+    const int h = U.j / A.tiles;
+    combine<DT>(A, lds, parts_of(R, U), U.b, h, U.j - h * A.tiles);
 }
 
 template <int NS>
@@ -481,12 +627,11 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs& A, int dt, hipStream_t stream) {
     const void* f = table[A.c.ns - 1](dt);
     Kv4AttnArgs a = A;
     void* args[] = {&a};
-    const dim3 units(1, A.c.heads * A.tiles, A.c.seqs);
-    hipError_t e = launch(f, dim3(A.splits, units.y, units.z), dim3(64 * WAVES), args, 0, stream);
-    if (e != hipSuccess || A.splits == 1 || A.split_cnt) return e;
+    hipError_t e = launch(f, dim3(A.groups), dim3(64 * WAVES), args, 0, stream);
+    if (e != hipSuccess || !A.partial || A.split_cnt) return e;
     f = dt == DT_F16 ? (const void*)kv4_combine_kernel<DT_F16>
       : dt == DT_BF16 ? (const void*)kv4_combine_kernel<DT_BF16> : (const void*)kv4_combine_kernel<DT_F32>;
-    return launch(f, units, dim3(64 * WAVES), args, 0, stream);
+    return launch(f, dim3(A.groups), dim3(64 * WAVES), args, 0, stream);
 }
 
 }  // namespace cbk

@@ -108,7 +108,7 @@ def _attention(**kw):
     (dict(d=4), "head_dim must be"), (dict(scale=0.0), "scale must be"), (dict(scale=-1.0), "scale must be"),
     (dict(scale=float("nan")), "scale must be"), (dict(scale=float("inf")), "scale must be"), (dict(t=-1), "new tokens"),
     (dict(t=1 << 22), "too many new tokens"), (dict(q=None), "non-null"), (dict(out=ALIGNED + 4), "16-byte aligned"),
-    (dict(floats=0, width=64), "partial must hold"), (dict(partial=None, width=64), "partial must hold"),
+    (dict(seqs=60000, width=100000), "block table too wide"), (dict(floats=0, width=64), "partial must hold"), (dict(partial=None, width=64), "partial must hold"),
     (dict(lens=None), "non-null"), (dict(page=100), "page_size must be"),
 ])
 def test_attention_refusals(kw, msg):
@@ -117,9 +117,10 @@ def test_attention_refusals(kw, msg):
 
 def test_partial_floats():
     n = lib.cbk_kv4_attention_partial_floats
-    assert n(1, 1, 32, 8, 128, 64, 1) == 0                      # two blocks: one workgroup
-    assert n(64, 1, 32, 32, 128, 64, 64) == 0                   # sequences and heads fill the chip
-    assert n(1, 1, 32, 8, 128, 64, 64) % (8 * 4 * 130) == 0 and n(1, 1, 32, 8, 128, 64, 64) > 0
+    assert n(1, 1, 32, 8, 128, 64, 1) == 0                      # units of two blocks are never cut
+    for seqs, width in ((1, 64), (64, 64), (1, 2048)):          # two slots a workgroup of rows of sums and two more
+        got = n(seqs, 1, 32, 8, 128, 64, width)
+        assert got > 0 and got % (2 * 4 * 130) == 0
     for bad in ((0, 1, 32, 8, 128, 64, 64), (1, 1, 3, 2, 128, 64, 64), (1, 1, 2, 2, 12, 64, 64), (1, 1, 2, 2, 128, 48, 64)):
         assert n(*bad) == 0
 
