@@ -7,7 +7,7 @@
  *
  * Types: dtype (CBK_F16 / CBK_BF16 / CBK_F32) is that of q, k, v and the outputs.  head_dim is a multiple of 8
  * up to 256.  Query head h reads kv head h / (heads / kv_heads).  Pointers to q, k, v and outputs are 16-byte
- * aligned and so is every row of a head (strides in elements).
+ * aligned and so is every row of a head (strides in elements, between rows at most 2^23).
  *
  * The cache.  pages is int32 [num_pages, kv_heads, cbk_kv4_page_words(head_dim, page_size)], 16-byte
  * aligned; page_size a power of two from 32 on.  Token i of sequence b lies in page

@@ -17,6 +17,8 @@ namespace {
 constexpr int64_t MOST = INT32_MAX / 2;        // rows, pages, tokens of a table: positions stay in 32 bits
 constexpr int64_t MOST_GRID = 65535;           // the second and third grid dimension
 
+constexpr int64_t MAX_ROW_STRIDE = 1 << 23;
+
 bool valid_dtype(int dt) { return dt == CBK_F16 || dt == CBK_BF16 || dt == CBK_F32; }
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int esize(int dt) { return dt == CBK_F32 ? 4 : 2; }
@@ -30,11 +32,12 @@ int check_heads(const char* what, int dtype, int64_t heads, int64_t kv_heads, in
     return CBK_OK;
 }
 
-// 16-byte rows of a head: a stride that the kernels step by with vector accesses.
+// 16-byte rows of a head: strides that the kernels step by with vector accesses (and 32-bit offsets within 64 rows).
 int check_strides(const char* what, int dtype, int64_t row, int64_t head) {
     const int64_t unit = 16 / esize(dtype);
     if (row < 0 || head < 0 || row % unit != 0 || head % unit != 0)
         return fail(CBK_EINVAL, "%s: rows of a head must be 16-byte aligned", what);
+    if (row > MAX_ROW_STRIDE) return fail(CBK_EINVAL, "%s: row strides are at most 2^23 elements", what);
     return CBK_OK;
 }
 

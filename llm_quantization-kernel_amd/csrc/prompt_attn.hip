@@ -58,14 +58,20 @@ __device__ __forceinline__ f16v zero16() {
 }
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef const __attribute__((address_space(1))) void* glb_ptr;
+typedef const __attribute__((address_space(3))) u4* lds_u4;
+typedef __attribute__((address_space(3))) s4* lds_s4;
 
-// Position (in 16-byte chunks) of chunk c of row r in a tile of CP chunks a row.  K: a wave's reads take two
-// neighbouring chunks of 32 rows; V: four neighbouring chunks of eight rows.  Both orders spread them over the banks.
+// In LDS a row of CP 16-byte chunks keeps chunk c of row r at c ^ k_turn(r) or c ^ v_turn(r).  A wave reads, of K, two
+// neighbouring chunks of 32 rows at once, of V four neighbouring chunks of eight rows: with these turns either
+// covers the 64 banks evenly.
 template <int CP>
-__device__ __forceinline__ int k_at(int r, int c) { return r * CP + (c ^ (r & (CP - 1))); }
+__device__ __forceinline__ int k_turn(int r) {
+    return CP >= 16 ? (r & 7) << 1 : CP == 8 ? (r >> 1 & 3) << 1 : (r >> 2 & 1) << 1;
+}
 template <int CP>
-__device__ __forceinline__ int v_at(int r, int c) { return r * CP + (c ^ ((r & 3) << 2 & (CP - 1))); }
+__device__ __forceinline__ int v_turn(int r) {
+    return CP >= 16 ? (r & 3) << 2 : CP == 8 ? (r >> 1 & 1) << 2 : 0;
+}
 
 // KS: steps of 16 of the head's values, DT32: tiles of 32, CP: chunks of a row in LDS.
 template <int DT, int KS, int CP>
@@ -119,24 +125,29 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
             q[s] = c < chunks ? *reinterpret_cast<const u4*>(qp + 8 * c) : u4{0, 0, 0, 0};
         }
     }
-    // K steps past the head's values: zeros in both buffers
-    for (int c = chunks; c < 2 * KS; ++c)
-        for (int x = threadIdx.x; x < 2 * KT; x += 64 * WAVES)
-            *reinterpret_cast<u4*>(lds + (x / KT) * 2 * TILE + 16 * k_at<CP>(x % KT, c)) = u4{0, 0, 0, 0};
-
+    // Staging: each lane brings 16-byte chunks, its place in the tile fixed by the lane; rows behind the sequence and chunks
+    // behind the head's values are out of the buffer's range and come as zeros.
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)lds;
+    constexpr int LOADS = KT * CP / (64 * WAVES), STEP = 64 * WAVES / CP;      // loads of a lane, rows between them
+    const uint32_t k_bytes = (uint32_t)A.k_row * 2, v_bytes = (uint32_t)A.v_row * 2;
+    uint32_t k_off, v_off;
+    {
+        const int pos = wave * 64 + lane, r = pos / CP, c = pos % CP;
+        const int ck = c ^ k_turn<CP>(r), cv = c ^ v_turn<CP>(r);
+        k_off = ck < chunks ? r * k_bytes + 16 * ck : 0x7FFFFFF0u;
+        v_off = cv < chunks ? r * v_bytes + 16 * cv : 0x7FFFFFF0u;
+    }
     auto stage = [&](int t, int buf) {
+        const long left = len - t * KT;
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(kp + (long)t * KT * A.k_row), 0, (int)min((left - 1) * k_bytes + 2 * D, 0x7FFFFF00l), 0x00020000);
+        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(vp + (long)t * KT * A.v_row), 0, (int)min((left - 1) * v_bytes + 2 * D, 0x7FFFFF00l), 0x00020000);
+        const uint32_t to = lds0 + buf * 2 * TILE + wave * 1024;
 #pragma unroll
-        for (int i = 0; i < KT * CP / (64 * WAVES); ++i) {
-            const int pos = (i * WAVES + wave) * 64 + lane;       // chunk position in the tile
-            const int r = pos / CP, cx = pos % CP;
-            const int tok = min(t * KT + r, len - 1);
-            char* to = lds + buf * 2 * TILE + (i * WAVES + wave) * 1024;
-            const int ck = cx ^ (r & (CP - 1)), cv = cx ^ ((r & 3) << 2 & (CP - 1));
-            if (ck < chunks)
-                __builtin_amdgcn_global_load_lds((glb_ptr)(kp + (long)tok * A.k_row + 8 * ck), (lds_ptr)to, 16, 0, 0);
-            if (cv < chunks)
-                __builtin_amdgcn_global_load_lds((glb_ptr)(vp + (long)tok * A.v_row + 8 * cv), (lds_ptr)(to + TILE),
-                                                 16, 0, 0);
+        for (int i = 0; i < LOADS; ++i) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr)(to + i * WAVES * 1024), 16, k_off, i * STEP * k_bytes, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr)(to + TILE + i * WAVES * 1024), 16, v_off, i * STEP * v_bytes, 0, 0);
         }
     };
 
@@ -146,33 +157,47 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
     float M = LOW, l = 0.f;
     const float cc = A.scale * 1.44269504088896341f;
 
-    // V^T operand of d tile i, token step s: two transposed reads of four tokens
+    // LDS addresses of this lane's operands: K row n (32 rows on: the same turn), step s at `k_lds ^ 32 s`; V^T of d tile i
+    // at `v_lds ^ 64 i`, two transposed reads of four tokens a token step.
+    const uint32_t k_lds = lds0 + 16 * (n * CP + (hf ^ k_turn<CP>(n)));
     const int tr_row = 4 * hf + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const int tr_byte = 8 * (lane & 1);
-    auto v_operand = [&](const char* vt, int i, int s) {
+    const uint32_t v_lds = lds0 + TILE + 16 * (tr_row * CP + (tr_chunk ^ v_turn<CP>(tr_row))) + 8 * (lane & 1);
+    auto k_operand = [&](int buf, int i, int s) {
+        return *reinterpret_cast<lds_u4>((k_lds ^ (32 * s)) + (buf * 2 * TILE + i * 32 * CP * 16));
+    };
+    auto v_operand = [&](int buf, int i, int s) {
         union { s4 h[2]; u4 v; } o;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const int r = 16 * s + 8 * p + tr_row;
-            const char* at = vt + 16 * v_at<CP>(r, 4 * i + tr_chunk) + tr_byte;
-            o.h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
-        }
+        for (int p = 0; p < 2; ++p)
+            o.h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                reinterpret_cast<lds_s4>((v_lds ^ (64 * i)) + (buf * 2 * TILE + (16 * s + 8 * p) * CP * 16)));
         return o.v;
     };
 
     bool odd_values = false;                                      // some V tile on the diagonal is not all finite
-    auto tile_step = [&](int t, auto edge_tag) {
+    auto tile_step = [&](int t, auto buf_tag, auto edge_tag) {
+        constexpr int BUF = decltype(buf_tag)::value;
         constexpr bool EDGE = decltype(edge_tag)::value;          // some row does not see all of the tile
-        const char* kt = lds + (t & 1) * 2 * TILE;
-        const char* vt = kt + TILE;
+        bool finite = true;
+        if constexpr (EDGE) {
+            // V times zeros: NaN where some value is an infinity or NaN
+            f16v test = zero16();
+#pragma unroll
+            for (int i = 0; i < DT32; ++i)
+#pragma unroll
+                for (int st = 0; st < 4; ++st) test = mfma<DT>(v_operand(BUF, i, st), u4{0, 0, 0, 0}, test);
+            float any = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) any += test[j];
+            finite = __builtin_amdgcn_ballot_w64(any != any) == 0;
+        }
         f16v s[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            s[i] = zero16();
+        for (int i = 0; i < 2; ++i) s[i] = zero16();
 #pragma unroll
-            for (int st = 0; st < KS; ++st)
-                s[i] = mfma<DT>(*reinterpret_cast<const u4*>(kt + 16 * k_at<CP>(32 * i + n, 2 * st + hf)), q[st], s[i]);
-        }
+        for (int st = 0; st < KS; ++st)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s[i] = mfma<DT>(k_operand(BUF, i, st), q[st], s[i]);
         if constexpr (EDGE) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -187,7 +212,11 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
-        top = fmaxf(top, __shfl_xor(top, 32)) * cc;
+        {
+            const uint32_t u = __float_as_uint(top);
+            const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * cc;
+        }
         if (__builtin_amdgcn_ballot_w64(top > M + SLACK) != 0) {
             const float to = top > M + SLACK ? top : M;
             const float f = __builtin_amdgcn_exp2f(M - to);
@@ -209,21 +238,13 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
                 w[2 * i + (j >> 3)][(j & 7) >> 1] = pack2<DT>(x, y);
             }
         if constexpr (EDGE) {
-            uint32_t bad = 0;
-            for (int x = lane; x < KT * CP; x += 64) {
-                const int r = x / CP, c = (x % CP) ^ ((r & 3) << 2 & (CP - 1));
-                if (c >= chunks) continue;
-                const u4 v = *reinterpret_cast<const u4*>(vt + 16 * x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) bad |= not_finite(v[e]);
-            }
-            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+            if (!finite) {
                 odd_values = true;
 #pragma unroll
                 for (int i = 0; i < DT32; ++i)
 #pragma unroll
                     for (int st = 0; st < 4; ++st) {
-                        u4 v = v_operand(vt, i, st);
+                        u4 v = v_operand(BUF, i, st);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] &= ~not_finite(v[e]);
                         acc[i] = mfma<DT>(v, w[st], acc[i]);
@@ -232,20 +253,25 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
             }
         }
 #pragma unroll
-        for (int i = 0; i < DT32; ++i)
+        for (int st = 0; st < 4; ++st)
 #pragma unroll
-            for (int st = 0; st < 4; ++st) acc[i] = mfma<DT>(v_operand(vt, i, st), w[st], acc[i]);
+            for (int i = 0; i < DT32; ++i) acc[i] = mfma<DT>(v_operand(BUF, i, st), w[st], acc[i]);
     };
 
     const int tiles = (min(q0 + ROWS, len) + KT - 1) / KT;       // the workgroup's last row sees up to itself
     const int whole = (wq + 1) / KT;                              // tiles that every row of this wave sees all of
     stage(0, 0);
-    for (int t = 0; t < tiles; ++t) {
+    auto turn = [&](int t, auto buf_tag) {
         __syncthreads();                                          // tile t has landed; tile t - 1 has been read
-        if (t + 1 < tiles) stage(t + 1, (t + 1) & 1);
-        if (t < whole) tile_step(t, std::integral_constant<bool, false>{});
-        else if (t * KT <= wq + 31) tile_step(t, std::integral_constant<bool, true>{});
+        if (t + 1 < tiles) stage(t + 1, 1 - decltype(buf_tag)::value);
+        if (t < whole) tile_step(t, buf_tag, std::integral_constant<bool, false>{});
+        else if (t * KT <= wq + 31) tile_step(t, buf_tag, std::integral_constant<bool, true>{});
+    };
+    for (int t = 0; t < tiles; t += 2) {
+        turn(t, std::integral_constant<int, 0>{});
+        if (t + 1 < tiles) turn(t + 1, std::integral_constant<int, 1>{});
     }
+
     l += __shfl_xor(l, 32);
     if (row >= len) return;
     const float inv = 1.f / l;

@@ -38,6 +38,7 @@ Tensor rows_of(const Tensor& t) {
     const int64_t unit = 16 / t.element_size();
     bool fits = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     for (int64_t i = 0; i + 1 < t.dim(); ++i) fits = fits && t.stride(i) >= 0 && (t.size(i) <= 1 || t.stride(i) % unit == 0);
+    fits = fits && (t.size(0) <= 1 || t.stride(0) <= (1 << 23));
     return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 

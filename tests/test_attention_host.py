@@ -134,7 +134,7 @@ def _prompt(**kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(dtype=4), "fp16/bf16/fp32"), (dict(heads=5), "multiple of kv_heads"), (dict(d=100), "head_dim must be"),
-    (dict(qr=510), "16-byte aligned"), (dict(kh=4), "16-byte aligned"), (dict(vr=-8), "16-byte aligned"),
+    (dict(qr=510), "16-byte aligned"), (dict(kr=1 << 24), "at most 2^23"), (dict(kh=4), "16-byte aligned"), (dict(vr=-8), "16-byte aligned"),
     (dict(v=ALIGNED + 8), "16-byte aligned"), (dict(cu=None), "non-null"), (dict(out=None), "non-null"),
     (dict(scale=0.0), "scale must be"), (dict(longest=0), "max_seqlen must be"), (dict(longest=101), "max_seqlen must be"),
     (dict(seqs=0), "rows without a sequence"), (dict(seqs=70000), "at most"), (dict(rows=-5), "number of rows"),
