@@ -10,8 +10,8 @@
 // largest score exceeds it by 8 (w < 2^8 then, in range of fp16; sums are fp32).
 //
 // Masked places take no part whatever they hold: scores there are selected away, and a V tile on the diagonal
-// that has infinities or NaN (a product 0 x inf would reach rows that do not see it) is taken with those values
-// zeroed, and what a row sees of them is added at the end.
+// that has infinities or NaN (a product 0 x inf would reach rows that do not see it) is left for a second pass, with those
+// values zeroed, and what a row sees of them is added at the end.
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
 
@@ -174,11 +174,12 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
         return o.v;
     };
 
-    bool odd_values = false;                                      // some V tile on the diagonal is not all finite
+    const int tiles = (min(q0 + ROWS, len) + KT - 1) / KT;       // the workgroup's last row sees up to itself
+    const int whole = (wq + 1) / KT;                              // tiles that every row of this wave sees all of
+    uint32_t odd = 0;                                             // tiles from `whole` on whose V is not all finite
     auto tile_step = [&](int t, auto buf_tag, auto edge_tag) {
         constexpr int BUF = decltype(buf_tag)::value;
         constexpr bool EDGE = decltype(edge_tag)::value;          // some row does not see all of the tile
-        bool finite = true;
         if constexpr (EDGE) {
             // V times zeros: NaN where some value is an infinity or NaN
             f16v test = zero16();
@@ -189,7 +190,10 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
             float any = 0.f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) any += test[j];
-            finite = __builtin_amdgcn_ballot_w64(any != any) == 0;
+            if (__builtin_amdgcn_ballot_w64(any != any) != 0) {
+                odd |= 1u << (t - whole);
+                return;
+            }
         }
         f16v s[2];
 #pragma unroll
@@ -237,39 +241,51 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
                 l += x + y;
                 w[2 * i + (j >> 3)][(j & 7) >> 1] = pack2<DT>(x, y);
             }
-        if constexpr (EDGE) {
-            if (!finite) {
-                odd_values = true;
-#pragma unroll
-                for (int i = 0; i < DT32; ++i)
-#pragma unroll
-                    for (int st = 0; st < 4; ++st) {
-                        u4 v = v_operand(BUF, i, st);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] &= ~not_finite(v[e]);
-                        acc[i] = mfma<DT>(v, w[st], acc[i]);
-                    }
-                return;
-            }
-        }
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
             for (int i = 0; i < DT32; ++i) acc[i] = mfma<DT>(v_operand(BUF, i, st), w[st], acc[i]);
     };
 
-    const int tiles = (min(q0 + ROWS, len) + KT - 1) / KT;       // the workgroup's last row sees up to itself
-    const int whole = (wq + 1) / KT;                              // tiles that every row of this wave sees all of
-    stage(0, 0);
+    // All tiles, then, where some wave left tiles out, the diagonal ones again with V's infinities and NaN as zeros.
+    bool again = false;
     auto turn = [&](int t, auto buf_tag) {
+        constexpr int BUF = decltype(buf_tag)::value;
         __syncthreads();                                          // tile t has landed; tile t - 1 has been read
-        if (t + 1 < tiles) stage(t + 1, 1 - decltype(buf_tag)::value);
-        if (t < whole) tile_step(t, buf_tag, std::integral_constant<bool, false>{});
-        else if (t * KT <= wq + 31) tile_step(t, buf_tag, std::integral_constant<bool, true>{});
+        if (again) {
+            for (int x = threadIdx.x; x < KT * CP; x += 64 * WAVES) {
+                u4* at = reinterpret_cast<u4*>(lds + (2 * BUF + 1) * TILE) + x;
+                u4 v = *at;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] &= ~not_finite(v[e]);
+                *at = v;
+            }
+            __syncthreads();
+        }
+        if (t + 1 < tiles) stage(t + 1, 1 - BUF);
+        if (again ? t >= whole && (odd >> (t - whole) & 1) : t >= whole && t * KT <= wq + 31)
+            tile_step(t, buf_tag, std::integral_constant<bool, true>{});
+        else if (!again && t < whole)
+            tile_step(t, buf_tag, std::integral_constant<bool, false>{});
     };
-    for (int t = 0; t < tiles; t += 2) {
-        turn(t, std::integral_constant<int, 0>{});
-        if (t + 1 < tiles) turn(t + 1, std::integral_constant<int, 1>{});
+    for (int t0 = 0;;) {
+        stage(t0, 0);
+        for (int t = t0; t < tiles; t += 2) {
+            turn(t, std::integral_constant<int, 0>{});
+            if (t + 1 < tiles) turn(t + 1, std::integral_constant<int, 1>{});
+        }
+        if (again) break;
+        __syncthreads();                                          // the tiles have been read: the waves' marks go there
+        uint32_t* marks = reinterpret_cast<uint32_t*>(lds);
+        if (lane == 0) marks[wave] = odd;
+        __syncthreads();
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) any |= marks[i];
+        if (!any) break;
+        __syncthreads();
+        again = true;
+        t0 = (q0 + 1) / KT;
     }
 
     l += __shfl_xor(l, 32);
@@ -288,7 +304,7 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
                 *reinterpret_cast<uint2*>(o + d) = v;
             }
         }
-    if (odd_values) {                                             // what the row sees of them
+    if (odd) {                                                    // what the row sees of them
 #pragma unroll 1
         for (int tok = whole * KT; tok <= row; ++tok)
 #pragma unroll 1
