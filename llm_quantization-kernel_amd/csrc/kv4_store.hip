@@ -4,13 +4,14 @@
 // hi = max(0, max x), r = hi - lo and z = rint(-15 lo / r) in 64 bits, the word
 // (bits(max(float(r / 15), 2^-100)) & ~15) | z, whose float is s, and c = clamp(rint(x / s) + z, 0, 15)
 // with x / s at its exact value (halves to even).  The codes follow the definition exactly, at borders too:
-// a rounded quotient would move a whole step.  rint(x * (1 / s)) is off by at most one, and
-// e = x - q s, exact in one FMA where it matters (near s / 2 it is a multiple of half x's last place
-// below 2^24 of them), says which way.
+// a rounded quotient would move a whole step.  x * (1 / s) is off by less than 2e-6, so its rint is right
+// unless it lies within 4e-6 of a half; where some lane's does (one wave pass in a few hundred) e = x - q s decides,
+// exact in one FMA there (a multiple of half x's last place below 2^24 of them).  z is found the same way.
 //
 // A wave has one block of 32 tokens of one head.  K: 16 lanes (32 above 128 values) hold a token, eight
-// values each, and write one word each.  V's words hold eight tokens of one value: the codes pass
-// through LDS as bytes [value][token].  A block that is not all new keeps the other tokens' codes.
+// values each, and write one word each; the next four tokens' loads are under way meanwhile.  V's words hold eight
+// tokens of one value: the codes pass through LDS as bytes [value][token], and a word is two dwords of them folded
+// together.  A block that is not all new keeps the other tokens' codes (read ahead of the rest).
 // Bound: the bytes (the 16-bit values in, codes out).
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
@@ -60,32 +61,31 @@ __device__ __forceinline__ Where where_of(const Kv4View& C, const Kv4Rows& R, in
     return w;
 }
 
-// x / s rounded to the nearest whole number (halves to even), exactly, for |x / s| < 2^22.
-__device__ __forceinline__ float exact_quotient(float x, float s, float inv) {
-    float q = __builtin_rintf(x * inv);
-    const float e = __builtin_fmaf(-q, s, x), half = 0.5f * s;
-    const bool odd = ((int)q & 1) != 0;
-    if (e > half || (e == half && odd)) q += 1.f;
-    if (e < -half || (e == -half && odd)) q -= 1.f;
-    return q;
+// The smaller, and the larger, of a value over the W lanes of a token.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+template <int W, bool MAX>
+__device__ __forceinline__ float row_best(float v) {
+    auto best = [](float a, float b) { return MAX ? fmaxf(a, b) : fminf(a, b); };
+    v = best(v, dpp<0xB1>(v));          // lanes 1 apart, 2 apart, the other four of eight, the other eight
+    v = best(v, dpp<0x4E>(v));
+    v = best(v, dpp<0x141>(v));
+    v = best(v, dpp<0x140>(v));
+    if constexpr (W == 32) {
+        const uint32_t u = __float_as_uint(v);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        v = best(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return v;
 }
 
-template <int W>
-__device__ __forceinline__ float row_min(float v) {
-#pragma unroll
-    for (int m = 1; m < W; m <<= 1) v = fminf(v, __shfl_xor(v, m));
-    return v;
-}
-template <int W>
-__device__ __forceinline__ float row_max(float v) {
-#pragma unroll
-    for (int m = 1; m < W; m <<= 1) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
-}
+constexpr float NEAR_HALF = 0.5f - 4e-6f;
 
 // Eight values of a vector spread over W lanes -> their codes and the vector's word.
 template <int W>
-__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], int (&c)[8]) {
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], int lane, int (&c)[8]) {
     float lo = 0.f, hi = 0.f;
     bool fine = true;
 #pragma unroll
@@ -94,23 +94,47 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], int (&c)[8]) 
         hi = fmaxf(hi, x[j]);
         fine &= __builtin_fabsf(x[j]) < __builtin_inff();
     }
-    lo = row_min<W>(lo);
-    hi = row_max<W>(hi);
-    const float bad = row_max<W>(fine ? 0.f : 1.f);
+    lo = row_best<W, false>(lo);
+    hi = row_best<W, true>(hi);
+    const uint64_t odd = __builtin_amdgcn_ballot_w64(!fine);
     const double r = (double)hi - (double)lo;
-    const int z = r > 0.0 ? (int)__builtin_rint(-15.0 * (double)lo / r) : 0;
-    const float step = fmaxf((float)(r / 15.0), KV4_MIN_SCALE);
+    // z = rint(-15 lo / r), near 0 .. 15; r / 15 by its reciprocal and one correction, which rounds as the division
+    const float zt = -15.f * ((float)((double)lo * 0x1p-64) / (float)(r * 0x1p-64));
+    float zr = r > 0.0 ? __builtin_rintf(zt) : 0.f;
+    if (__builtin_amdgcn_ballot_w64(r > 0.0 && !(__builtin_fabsf(zt - zr) < NEAR_HALF)) != 0)
+        zr = r > 0.0 ? (float)__builtin_rint(-15.0 * (double)lo / r) : 0.f;
+    const double fifteenth = 1.0 / 15.0, q0 = r * fifteenth;
+    const double fifth = __builtin_fma(__builtin_fma(-15.0, q0, r), fifteenth, q0);
+    const float step = fmaxf((float)fifth, KV4_MIN_SCALE);
+    const int z = (int)zr;
     uint32_t word = (__float_as_uint(step) & ~15u) | (uint32_t)z;
     const float s = __uint_as_float(word), inv = 1.0f / s;
+    float q[8], far = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float q = exact_quotient(x[j], s, inv) + (float)z;
-        c[j] = (int)fminf(fmaxf(q, 0.f), 15.f);
+        const float t = x[j] * inv;
+        q[j] = __builtin_rintf(t);
+        far = fmaxf(far, __builtin_fabsf(t - q[j]));
     }
-    if (bad != 0.f) {
-        word = 0x7FC00000u;
+    if (__builtin_amdgcn_ballot_w64(!(far < NEAR_HALF)) != 0) {
+        const float half = 0.5f * s;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = 0;
+        for (int j = 0; j < 8; ++j) {
+            const float e = __builtin_fmaf(-q[j], s, x[j]);
+            const bool uneven = ((int)q[j] & 1) != 0;
+            const bool up = e > half || (e == half && uneven), down = e < -half || (e == -half && uneven);
+            q[j] += up ? 1.f : down ? -1.f : 0.f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = (int)fminf(fmaxf(q[j] + zr, 0.f), 15.f);
+    if (odd) {
+        const uint64_t own = (W == 32 ? 0xFFFFFFFFull : 0xFFFFull) << (lane & ~(W - 1));
+        if (odd & own) {
+            word = 0x7FC00000u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j] = 0;
+        }
     }
     return word;
 }
@@ -169,62 +193,85 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_append_kernel(Kv4StoreArgs A, 
     if (!base) return;
     const int ns = C.ns, sub = lane / W, i8 = lane % W;      // token of the pass, word of the token
     const bool mine = 8 * i8 < C.d;
+    const int psh = ns & 1 ? 1 : 2;                    // log2 of the words of a piece
     uint32_t* meta = base + 256 * ns;
+    uint32_t* vc = base + 128 * ns;
     uint8_t* lds = codes[wave];
-    for (int t0 = 32 * blk; t0 < 32 * blk + 32; t0 += TOK) {
-        if (t0 + TOK <= lo || t0 >= hi) continue;
+    const bool part = hi - lo < 32;
+    uint32_t old[KV4_MAX_D / 16 * W / 32];             // V's words of a block that keeps some (2 ns of them a lane)
+    if (part) {
+#pragma unroll
+        for (int i = 0; i < KV4_MAX_D / 16 * W / 32; ++i)
+            if (i < 2 * ns) old[i] = vc[lane + 64 * i];
+    }
+    // values of the pass at t0 (the nearest rows that are new where the lane's own is not)
+    const long k0 = h * A.k_head + (mine ? 8 * i8 : 0), v0 = h * A.v_head + (mine ? 8 * i8 : 0);
+    auto fetch = [&](int t0, float (&xk)[8], float (&xv)[8]) {
+        const long row = w.row0 + (min(max(t0 + sub, lo), hi - 1) - w.pos0);
+        load8<DT>(A.k, row * A.k_row + k0, xk);
+        load8<DT>(A.v, row * A.v_row + v0, xv);
+    };
+    const int from = 32 * blk + (lo - 32 * blk) / TOK * TOK;
+    float xk[8], xv[8], nk[8], nv[8];
+    fetch(from, xk, xv);
+    for (int t0 = from; t0 < hi; t0 += TOK) {
+        fetch(t0 + TOK, nk, nv);
         const int pos = t0 + sub, tok = pos - 32 * blk;
         const bool is_new = pos >= lo && pos < hi;
-        float xk[8] = {}, xv[8] = {};
-        if (is_new && mine) {
-            const long row = w.row0 + (pos - w.pos0);
-            load8<DT>(A.k, row * A.k_row + h * A.k_head + 8 * i8, xk);
-            load8<DT>(A.v, row * A.v_row + h * A.v_head + 8 * i8, xv);
-        }
         int c[8];
-        const uint32_t kw = quantize8<W>(xk, c);
-        if (!mine) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) c[j] = 0;
-        }
+        for (int j = 0; j < 8; ++j) xk[j] = mine ? xk[j] : 0.f, xv[j] = mine ? xv[j] : 0.f;
+        const uint32_t kw = quantize8<W>(xk, lane, c);
         if (is_new) {
             if (i8 < 4 * ns) {
                 uint32_t word = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) word |= kv4_put((uint32_t)c[j], j);
+                for (int j = 0; j < 8; ++j) word |= mine ? kv4_put((uint32_t)c[j], j) : 0u;
                 base[tok * 4 * ns + i8] = word;
             }
             if (i8 == 0) meta[tok] = kw;
         }
-        const uint32_t vw = quantize8<W>(xv, c);
-        if (!mine) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) c[j] = 0;
-        }
+        const uint32_t vw = quantize8<W>(xv, lane, c);
         if (is_new && i8 == 0) meta[32 + tok] = vw;
         if (is_new && i8 < 4 * ns) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) lds[(8 * i8 + j) * PITCH + tok] = (uint8_t)c[j];
+            for (int j = 0; j < 8; ++j) lds[(8 * i8 + j) * PITCH + tok] = (uint8_t)(mine ? c[j] : 0);
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) xk[j] = nk[j], xv[j] = nv[j];
     }
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4));    // lgkmcnt(0): the wave's own bytes
     asm volatile("" ::: "memory");
-    const int psh = ns & 1 ? 1 : 2;                    // log2 of the words of a piece
-    uint32_t* vc = base + 128 * ns;
-    for (int x = lane; x < 128 * ns; x += 64) {
+#pragma unroll
+    for (int i = 0; i < KV4_MAX_D / 16 * W / 32; ++i) {
+        if (i >= 2 * ns) break;
+        const int x = lane + 64 * i;
         const int e = x & ((1 << psh) - 1), y = x >> psh;
         const int m = y & 15, g = (y >> 4) & 3, piece = y >> 6;
         const int d = 16 * ((piece << psh) + e) + m;
-        uint32_t keep = 0, word = 0;
+        // tokens 4 g + 0..3 and 16 + 4 g + 0..3 of value d, a byte each: fold them to nibbles (0, 2, 1, 3), and the
+        // two to the word's (0, 2, 4, 6, 1, 3, 5, 7), turned by two bits
+        auto fold = [](uint32_t a, uint32_t b) {
+            a &= 0x0F0F0F0Fu, b &= 0x0F0F0F0Fu;        // bytes of tokens that are not new hold anything
+            a |= a >> 12, b |= b >> 12;
+            const uint32_t v = __builtin_amdgcn_perm(b, a, 0x05010400u);
+            return __builtin_amdgcn_alignbit(v, v, 30);
+        };
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(lds + d * PITCH + 4 * g);
+        uint32_t word = fold(at[0], at[4]);
+        if (part) {
+            uint32_t na = 0, nb = 0;                   // which of the tokens are new
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int tok = 4 * g + (j & 3) + 16 * (j >> 2), pos = 32 * blk + tok;
-            if (pos >= lo && pos < hi) word |= kv4_put(lds[d * PITCH + tok], j);
-            else keep |= kv4_put(15u, j);
+            for (int j = 0; j < 4; ++j) {
+                const int pa = 32 * blk + 4 * g + j, pb = pa + 16;
+                na |= pa >= lo && pa < hi ? 15u << (8 * j) : 0u;
+                nb |= pb >= lo && pb < hi ? 15u << (8 * j) : 0u;
+            }
+            const uint32_t fresh = fold(na, nb);
+            if (fresh == 0) continue;
+            word = (word & fresh) | (old[i] & ~fresh);
         }
-        if (keep == 0xFFFFFFFFu) continue;
-        if (keep) word |= vc[x] & keep;
         vc[x] = word;
     }
 }
@@ -264,6 +311,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_read_kernel(Kv4StoreArgs A, in
     if (lo >= hi) return;
     const uint32_t* base = kv4_block(C, w.b, blk, h);
     const int psh = ns & 1 ? 1 : 2, pw = 1 << psh;
+#pragma unroll 4
     for (int t0 = 32 * blk; t0 < 32 * blk + 32; t0 += TOK) {
         const int pos = t0 + sub, tok = pos - 32 * blk;
         if (pos < lo || pos >= hi || !mine) continue;
