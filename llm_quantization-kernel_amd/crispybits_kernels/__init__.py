@@ -8,6 +8,7 @@ from .ops import (PackedLinearWeight, PackedLinear, packed_linear, fused_gate_up
 from .attention import KV4Cache, kv4_append, kv4_attention, kv4_read, prompt_attention
 from .autotune import tune_gemv, tune_qkv, tune_gate_up, tune_model, TuneResult, TuneReport
 from .io import from_packed_dict
-from .integration import install_bitmap, load_tuning, save_tuning, FusedQKV, FusedLlamaMLP
+from .integration import (install_attention, install_bitmap, kv4_cache, load_tuning, save_tuning, FusedQKV,
+                          FusedLlamaMLP)
 
 __version__ = "0.3.0+mi355x"

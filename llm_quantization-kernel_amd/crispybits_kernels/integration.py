@@ -272,10 +272,28 @@ def _block_file(packed_dir: Path, i: int, bits: int) -> Path:
     raise FileNotFoundError(f"neither block_{i:03d}_w{bits}.pt nor block_{i:03d}.pt in {packed_dir}")
 
 
+def install_attention(model: nn.Module) -> nn.Module:
+    """Make a Hugging Face causal LM attend through ``prompt_attention`` and, over a ``PagedKV4Cache`` given as
+    ``past_key_values``, ``kv4_attention`` (hf_attention.py says what it refuses)."""
+    from . import hf_attention
+    hf_attention.register()
+    model.set_attn_implementation(hf_attention.NAME)
+    return model
+
+
+def kv4_cache(model: nn.Module, max_batch_size: int, max_cache_len: int, page_size: int = 64, device=None):
+    """A ``PagedKV4Cache`` for the model, on its device unless another is given."""
+    from .hf_attention import PagedKV4Cache
+    if device is None:
+        device = next(model.parameters()).device
+    return PagedKV4Cache(model.config, max_batch_size, max_cache_len, device, page_size)
+
+
 def install_bitmap(model: nn.Module, packed_dir: str, bitmap, device="cuda", dtype=torch.float16,
-                   tuning: Optional[Dict] = None, fuse: bool = True, fuse_rope: bool = True):
+                   tuning: Optional[Dict] = None, fuse: bool = True, fuse_rope: bool = True, attention: bool = False):
     """Replace every linear of block i with its packed weights of width ``bitmap[i]`` (the
-    bitmap of ``manifest.json`` when None), then fuse each block's decode paths."""
+    bitmap of ``manifest.json`` when None), then fuse each block's decode paths; with ``attention``
+    the model also attends through this package's ops (``install_attention``)."""
     root = Path(packed_dir)
     if bitmap is None:
         with open(root / "manifest.json") as f:
@@ -299,7 +317,7 @@ def install_bitmap(model: nn.Module, packed_dir: str, bitmap, device="cuda", dty
         if fuse:
             for rule in _FUSIONS:
                 rule(block, i, tuning, fuse_rope)
-    return model
+    return install_attention(model) if attention else model
 
 
 def load_tuning(path: Optional[str]):
