@@ -392,7 +392,7 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
 
     // q scaled to below 2^11, and its sum
     Op q[TERMS][NS];
-    float cc, qsum = 0.f;
+    float cc, cl = 0.f, qsum = 0.f;
     {
         float x[NS][8];
         float top = 0.f;
@@ -428,7 +428,10 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                 if constexpr (!EXACT) qsum += (j & 2) ? held * 16.f : held;
             }
         if constexpr (!EXACT) qsum = group_sum(qsum) * 0x1p-22f;
-        cc = __builtin_ldexpf(A.scale * 1.44269504088896341f, UP - 11 + e);
+        // scale log2 e; for fp32 in two terms: its rounding would bend every score by 2^-24 of itself
+        const double c2 = (double)A.scale * 1.44269504088896340736;
+        cc = __builtin_ldexpf((float)c2, UP - 11 + e);
+        if constexpr (EXACT) cl = __builtin_ldexpf((float)(c2 - (double)(float)c2), UP - 11 + e);
     }
 
     f4 acc[TILES], accz = {0.f, 0.f, 0.f, 0.f};
@@ -485,7 +488,7 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
         float bound = ym * cc + (float)max(__builtin_amdgcn_frexp_expf(sm), -90);
         bound = group_max(bound);
         if (__builtin_amdgcn_ballot_w64(bound > M + SLACK) != 0) {
-            const float to = bound > M + SLACK ? bound : M;
+            const float to = bound > M + SLACK ? __builtin_ceilf(bound) : M;     // whole: what it scales stays exact
             const float f = __builtin_amdgcn_exp2f(M - to);
             M = to;
             la *= f, lb *= f;
@@ -500,7 +503,9 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
         float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, (j & 2) ? mb : ma));
+            float at = (j & 2) ? mb : ma;
+            if constexpr (EXACT) at = y[j] > -__builtin_inff() ? __builtin_fmaf(y[j], cl, at) : at;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, at));
             if (j & 2) lb += p;
             else la += p;
             w[j] = p * sv[j];

@@ -50,6 +50,12 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     }
 }
 
+// A value of the type (in the low half) as a float.
+template <int DT>
+__device__ __forceinline__ float half_of(uint32_t v) {
+    return Dt<DT>::to_f(__builtin_bit_cast(typename Dt<DT>::S, (uint16_t)v));
+}
+
 __device__ __forceinline__ f16v zero16() {
     f16v z;
 #pragma unroll
@@ -162,23 +168,23 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
     const uint32_t k_lds = lds0 + 16 * (n * CP + (hf ^ k_turn<CP>(n)));
     const int tr_row = 4 * hf + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     const uint32_t v_lds = lds0 + TILE + 16 * (tr_row * CP + (tr_chunk ^ v_turn<CP>(tr_row))) + 8 * (lane & 1);
-    auto k_operand = [&](int buf, int i, int s) {
-        return *reinterpret_cast<lds_u4>((k_lds ^ (32 * s)) + (buf * 2 * TILE + i * 32 * CP * 16));
+    auto k_operand = [&](uint32_t buf, int i, int s) {            // buf: the tile's buffer, in bytes
+        return *reinterpret_cast<lds_u4>(((k_lds + buf) ^ (32 * s)) + i * 32 * CP * 16);
     };
-    auto v_operand = [&](int buf, int i, int s) {
+    auto v_operand = [&](uint32_t buf, int i, int s) {
         union { s4 h[2]; u4 v; } o;
 #pragma unroll
         for (int p = 0; p < 2; ++p)
             o.h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                reinterpret_cast<lds_s4>((v_lds ^ (64 * i)) + (buf * 2 * TILE + (16 * s + 8 * p) * CP * 16)));
+                reinterpret_cast<lds_s4>(((v_lds + buf) ^ (64 * i)) + (16 * s + 8 * p) * CP * 16));
         return o.v;
     };
 
     const int tiles = (min(q0 + ROWS, len) + KT - 1) / KT;       // the workgroup's last row sees up to itself
     const int whole = (wq + 1) / KT;                              // tiles that every row of this wave sees all of
     uint32_t odd = 0;                                             // tiles from `whole` on whose V is not all finite
-    auto tile_step = [&](int t, auto buf_tag, auto edge_tag) {
-        constexpr int BUF = decltype(buf_tag)::value;
+    auto tile_step = [&](int t, auto edge_tag) {
+        const uint32_t BUF = (t & 1) * 2 * TILE;
         constexpr bool EDGE = decltype(edge_tag)::value;          // some row does not see all of the tile
         if constexpr (EDGE) {
             // V times zeros: NaN where some value is an infinity or NaN
@@ -195,84 +201,99 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
                 return;
             }
         }
-        f16v s[2];
+        // Two halves of 32 tokens: the second half's scores may run beside the first's weights, the first's sums beside the
+        // second's weights, and half a tile of scores is live at a time.
+        u4 w[4];                                                  // weights, 16 tokens a step
+        auto scores = [&](int i) {
+            f16v s = zero16();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = zero16();
-#pragma unroll
-        for (int st = 0; st < KS; ++st)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) s[i] = mfma<DT>(k_operand(BUF, i, st), q[st], s[i]);
-        if constexpr (EDGE) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int st = 0; st < KS; ++st) s = mfma<DT>(k_operand(BUF, i, st), q[st], s);
+            return s;
+        };
+        // masks what is not seen and moves M where a score is past it; `done`: steps of w that are scaled by it already
+        auto reference = [&](f16v& s, int i, int done) {
+            if constexpr (EDGE) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int tok = t * KT + 32 * i + 8 * (j >> 2) + 4 * hf + (j & 3);
-                    s[i][j] = tok <= row ? s[i][j] : -__builtin_inff();
+                    s[j] = tok <= row ? s[j] : -__builtin_inff();
                 }
-        }
-        float top = s[0][0];
+            }
+            float top = s[0];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
-        {
+            for (int j = 1; j < 16; ++j) top = fmaxf(top, s[j]);
             const uint32_t u = __float_as_uint(top);
             const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
             top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * cc;
-        }
-        if (__builtin_amdgcn_ballot_w64(top > M + SLACK) != 0) {
-            const float to = top > M + SLACK ? top : M;
-            const float f = __builtin_amdgcn_exp2f(M - to);
-            M = to;
-            l *= f;
+            if (__builtin_amdgcn_ballot_w64(top > M + SLACK) != 0) {
+                const float to = top > M + SLACK ? __builtin_ceilf(top) : M;       // whole: what it scales stays exact
+                const float f = __builtin_amdgcn_exp2f(M - to);
+                M = to;
+                l *= f;
 #pragma unroll
-            for (int i = 0; i < DT32; ++i)
+                for (int d = 0; d < DT32; ++d)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[i][j] *= f;
-        }
-        u4 w[4];                                                  // 16 tokens a step
+                    for (int j = 0; j < 16; ++j) acc[d][j] *= f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+                for (int k = 0; k < done; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[k][e] = pack2<DT>(half_of<DT>(w[k][e]) * f, half_of<DT>(w[k][e] >> 16) * f);
+            }
+        };
+        auto weights = [&](const f16v& s, int i) {
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], cc, -M));
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j + 1], cc, -M));
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cc, -M));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], cc, -M));
                 l += x + y;
                 w[2 * i + (j >> 3)][(j & 7) >> 1] = pack2<DT>(x, y);
             }
+        };
+        auto sums = [&](int i) {
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+            for (int st = 2 * i; st < 2 * i + 2; ++st)
 #pragma unroll
-            for (int i = 0; i < DT32; ++i) acc[i] = mfma<DT>(v_operand(BUF, i, st), w[st], acc[i]);
+                for (int d = 0; d < DT32; ++d) acc[d] = mfma<DT>(v_operand(BUF, d, st), w[st], acc[d]);
+        };
+        f16v s0 = scores(0);
+        reference(s0, 0, 0);
+        f16v s1 = scores(1);
+        weights(s0, 0);
+        reference(s1, 1, 2);
+        sums(0);
+        weights(s1, 1);
+        sums(1);
     };
 
     // All tiles, then, where some wave left tiles out, the diagonal ones again with V's infinities and NaN as zeros.
+    // Every turn has one barrier, so that waves may be in different loops.
     bool again = false;
-    auto turn = [&](int t, auto buf_tag) {
-        constexpr int BUF = decltype(buf_tag)::value;
+    auto turn = [&](int t) {
         __syncthreads();                                          // tile t has landed; tile t - 1 has been read
-        if (again) {
-            for (int x = threadIdx.x; x < KT * CP; x += 64 * WAVES) {
-                u4* at = reinterpret_cast<u4*>(lds + (2 * BUF + 1) * TILE) + x;
-                u4 v = *at;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] &= ~not_finite(v[e]);
-                *at = v;
-            }
-            __syncthreads();
-        }
-        if (t + 1 < tiles) stage(t + 1, 1 - BUF);
-        if (again ? t >= whole && (odd >> (t - whole) & 1) : t >= whole && t * KT <= wq + 31)
-            tile_step(t, buf_tag, std::integral_constant<bool, true>{});
-        else if (!again && t < whole)
-            tile_step(t, buf_tag, std::integral_constant<bool, false>{});
+        if (t + 1 < tiles) stage(t + 1, (t + 1) & 1);
     };
     for (int t0 = 0;;) {
-        stage(t0, 0);
-        for (int t = t0; t < tiles; t += 2) {
-            turn(t, std::integral_constant<int, 0>{});
-            if (t + 1 < tiles) turn(t + 1, std::integral_constant<int, 1>{});
+        stage(t0, t0 & 1);
+        int t = t0;
+        for (; !again && t < min(whole, tiles); ++t) {
+            turn(t);
+            tile_step(t, std::integral_constant<bool, false>{});
+        }
+        for (; t < tiles; ++t) {
+            if (again) {
+                __syncthreads();
+                for (int x = threadIdx.x; x < KT * CP; x += 64 * WAVES) {
+                    u4* at = reinterpret_cast<u4*>(lds + (2 * (t & 1) + 1) * TILE) + x;
+                    u4 v = *at;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] &= ~not_finite(v[e]);
+                    *at = v;
+                }
+            }
+            turn(t);
+            if (t >= whole && (again ? odd >> (t - whole) & 1 : t * KT <= wq + 31))
+                tile_step(t, std::integral_constant<bool, true>{});
         }
         if (again) break;
         __syncthreads();                                          // the tiles have been read: the waves' marks go there

@@ -66,7 +66,9 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
     float M = LOW, l = 0.f;
-    const float cc = A.scale * 1.44269504088896341f;
+    // scale log2 e in two terms: its rounding would bend every score by 2^-24 of itself
+    const double c2 = (double)A.scale * 1.44269504088896340736;
+    const float cc = (float)c2, cl = (float)(c2 - (double)cc);
     bool odd_values = false;
 
     const int last = min(q0 + ROWS, len);
@@ -95,6 +97,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
         }
         top = fmaxf(top, __shfl_xor(top, 32)) * cc;
         if (top > M) {
+            top = __builtin_ceilf(top);                 // whole: scores minus M and what M scales stay exact
             const float f = __builtin_amdgcn_exp2f(M - top);
             M = top;
             l *= f;
@@ -105,7 +108,8 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cc, -M));
+            const float at = s[j] > -__builtin_inff() ? __builtin_fmaf(s[j], cl, -M) : -M;
+            s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cc, at));
             l += s[j];
         }
         // masked places take no part whatever they hold: on the diagonal, infinities and NaN go in as zeros and

@@ -65,7 +65,13 @@ def test_long(hip, dtype):
 def test_one_token_and_none(hip, dtype):
     q, k, v, cu = _inputs([1], 4, 2, 128, dtype, 3)
     got = prompt_attention(q.cuda(), k.cuda(), v.cuda(), cu.cuda())
-    assert torch.equal(got.cpu(), v.repeat_interleave(2, 1))
+    want = v.repeat_interleave(2, 1)
+    if dtype == torch.float32:
+        # (w v)(1 / w) for a weight w in (1/2, 1]: three roundings, each at most 2^-24 of the value
+        assert ((got.cpu() - want).abs() <= 3.01 * 2.0 ** -24 * want.abs()).all()
+    else:
+        # a 16-bit w is off by at most half a step at its smallest mantissa, which v's own rounding takes back
+        assert torch.equal(got.cpu(), want)
     e = prompt_attention(q[:0].cuda(), k[:0].cuda(), v[:0].cuda(), torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert e.shape == (0, 4, 128)
 
