@@ -67,21 +67,35 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef const __attribute__((address_space(3))) u4* lds_u4;
 typedef __attribute__((address_space(3))) s4* lds_s4;
 
-// In LDS a row of CP 16-byte chunks keeps chunk c of row r at c ^ k_turn(r) or c ^ v_turn(r).  A wave reads, of K, two
-// neighbouring chunks of 32 rows at once, of V four neighbouring chunks of eight rows: with these turns either
-// covers the 64 banks evenly.
+// Where a tile's row r keeps its 16-byte chunk c, in chunks.  A wave reads, of K, two neighbouring chunks of 32 rows at
+// once, of V four neighbouring chunks of eight rows: either way the places cover the 64 banks evenly.  Rows have CP
+// chunks, a power of two, turned against each other by an exclusive or, or twelve (80 and 96 values: three
+// workgroups' tiles fit the LDS instead of two), whose pitch sets four rows apart by itself.
 template <int CP>
-__device__ __forceinline__ int k_turn(int r) {
-    return CP >= 16 ? (r & 7) << 1 : CP == 8 ? (r >> 1 & 3) << 1 : (r >> 2 & 1) << 1;
+__device__ __forceinline__ int k_place(int r, int c) {
+    if constexpr (CP == 12) return r * 12 + (c + 2 * (r >> 2 & 1)) % 12;
+    return r * CP + (c ^ (CP >= 16 ? (r & 7) << 1 : CP == 8 ? (r >> 1 & 3) << 1 : (r >> 2 & 1) << 1));
 }
 template <int CP>
-__device__ __forceinline__ int v_turn(int r) {
-    return CP >= 16 ? (r & 3) << 2 : CP == 8 ? (r >> 1 & 1) << 2 : 0;
+__device__ __forceinline__ int v_place(int r, int c) {
+    return r * CP + (c ^ (CP >= 16 ? (r & 3) << 2 : CP == 8 ? (r >> 1 & 1) << 2 : 0));
+}
+
+// A buffer over a sequence's rows (len of them, `stride` elements apart, D values each) from tile t on.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const uint16_t* base, long stride, int t, int len, int D) {
+    const long left = len - t * KT;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + (long)t * KT * stride), 0,
+                                             (int)min(((left - 1) * stride + D) * 2, 0x7FFFFF00l), 0x00020000);
+}
+
+// 16 bytes a lane from the buffer to LDS, the lanes' behind each other from `to` on.
+__device__ __forceinline__ void load_chunks(__amdgpu_buffer_rsrc_t from, uint32_t to, uint32_t offset, uint32_t rows) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)to, 16, offset, rows, 0, 0);
 }
 
 // KS: steps of 16 of the head's values, DT32: tiles of 32, CP: chunks of a row in LDS.
 template <int DT, int KS, int CP>
-__global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kernel(PromptArgs A, int row_tiles) {
+__global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void prompt_attn_kernel(PromptArgs A, int row_tiles) {
     constexpr int DT32 = (KS + 1) / 2;
     constexpr int TILE = KT * CP * 16;                 // bytes of a K or V tile
     auto not_finite = [](uint32_t v) {                 // all ones in each 16-bit half that is an infinity or NaN
@@ -134,26 +148,27 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
     // Staging: each lane brings 16-byte chunks, its place in the tile fixed by the lane; rows behind the sequence and chunks
     // behind the head's values are out of the buffer's range and come as zeros.
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)lds;
-    constexpr int LOADS = KT * CP / (64 * WAVES), STEP = 64 * WAVES / CP;      // loads of a lane, rows between them
+    // A lane's loads; where its chunks come from: the first's place, and the rows from one load to the next (turns are the
+    // same in all of them, twelve-chunk rows have a place for each).
+    constexpr int LOADS = KT * CP / (64 * WAVES), PLACES = CP == 12 ? LOADS : 1, STEP = CP == 12 ? 0 : 64 * WAVES / CP;
     const uint32_t k_bytes = (uint32_t)A.k_row * 2, v_bytes = (uint32_t)A.v_row * 2;
-    uint32_t k_off, v_off;
-    {
-        const int pos = wave * 64 + lane, r = pos / CP, c = pos % CP;
-        const int ck = c ^ k_turn<CP>(r), cv = c ^ v_turn<CP>(r);
-        k_off = ck < chunks ? r * k_bytes + 16 * ck : 0x7FFFFFF0u;
-        v_off = cv < chunks ? r * v_bytes + 16 * cv : 0x7FFFFFF0u;
+    uint32_t k_off[PLACES], v_off[PLACES];
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+        const int pos = (i * WAVES + wave) * 64 + lane, r = pos / CP, c = pos % CP;
+        // the chunk that is kept at place `pos`: a turn undoes itself, the rotation goes back
+        const int ck = CP == 12 ? (c + 12 - 2 * (r >> 2 & 1)) % 12 : k_place<CP>(r, c) - r * CP;
+        const int cv = v_place<CP>(r, c) - r * CP;
+        k_off[i] = ck < chunks ? r * k_bytes + 16 * ck : 0x7FFFFFF0u;
+        v_off[i] = cv < chunks ? r * v_bytes + 16 * cv : 0x7FFFFFF0u;
     }
     auto stage = [&](int t, int buf) {
-        const long left = len - t * KT;
-        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint16_t*>(kp + (long)t * KT * A.k_row), 0, (int)min((left - 1) * k_bytes + 2 * D, 0x7FFFFF00l), 0x00020000);
-        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint16_t*>(vp + (long)t * KT * A.v_row), 0, (int)min((left - 1) * v_bytes + 2 * D, 0x7FFFFF00l), 0x00020000);
+        const __amdgpu_buffer_rsrc_t kr = rows_from(kp, A.k_row, t, len, D), vr = rows_from(vp, A.v_row, t, len, D);
         const uint32_t to = lds0 + buf * 2 * TILE + wave * 1024;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr)(to + i * WAVES * 1024), 16, k_off, i * STEP * k_bytes, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr)(to + TILE + i * WAVES * 1024), 16, v_off, i * STEP * v_bytes, 0, 0);
+            load_chunks(kr, to + i * WAVES * 1024, k_off[i % PLACES], i * STEP * k_bytes);
+            load_chunks(vr, to + TILE + i * WAVES * 1024, v_off[i % PLACES], i * STEP * v_bytes);
         }
     };
 
@@ -163,20 +178,27 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : 2) void prompt_attn_kern
     float M = LOW, l = 0.f;
     const float cc = A.scale * 1.44269504088896341f;
 
-    // LDS addresses of this lane's operands: K row n (32 rows on: the same turn), step s at `k_lds ^ 32 s`; V^T of d tile i
-    // at `v_lds ^ 64 i`, two transposed reads of four tokens a token step.
-    const uint32_t k_lds = lds0 + 16 * (n * CP + (hf ^ k_turn<CP>(n)));
+    // LDS addresses of this lane's operands: K row n (32 rows on: the same places) at step s; V^T of d tile i, two
+    // transposed reads of four tokens a token step.  An exclusive or takes a turned row from step to step.
+    const uint32_t k_lds = lds0 + 16 * k_place<CP>(n, hf);
+    uint32_t k_step[CP == 12 ? KS : 1];
+    if constexpr (CP == 12)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) k_step[s] = lds0 + 16 * k_place<CP>(n, 2 * s + hf);
     const int tr_row = 4 * hf + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const uint32_t v_lds = lds0 + TILE + 16 * (tr_row * CP + (tr_chunk ^ v_turn<CP>(tr_row))) + 8 * (lane & 1);
+    const uint32_t v_lds = lds0 + TILE + 16 * v_place<CP>(tr_row, tr_chunk) + 8 * (lane & 1);
     auto k_operand = [&](uint32_t buf, int i, int s) {            // buf: the tile's buffer, in bytes
-        return *reinterpret_cast<lds_u4>(((k_lds + buf) ^ (32 * s)) + i * 32 * CP * 16);
+        uint32_t at;
+        if constexpr (CP == 12) at = k_step[s] + buf;
+        else at = (k_lds + buf) ^ (32 * s);
+        return *reinterpret_cast<lds_u4>(at + i * 32 * CP * 16);
     };
     auto v_operand = [&](uint32_t buf, int i, int s) {
+        const uint32_t at = CP == 12 ? v_lds + buf + 64 * i : (v_lds + buf) ^ (64 * i);
         union { s4 h[2]; u4 v; } o;
 #pragma unroll
         for (int p = 0; p < 2; ++p)
-            o.h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                reinterpret_cast<lds_s4>(((v_lds + buf) ^ (64 * i)) + (16 * s + 8 * p) * CP * 16));
+            o.h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4>(at + (16 * s + 8 * p) * CP * 16));
         return o.v;
     };
 
@@ -347,8 +369,8 @@ Built kernel_for(int d) {
         case 1: case 2: return {(const void*)prompt_attn_kernel<DT, 2, 4>, 4};
         case 3: return {(const void*)prompt_attn_kernel<DT, 3, 8>, 8};
         case 4: return {(const void*)prompt_attn_kernel<DT, 4, 8>, 8};
-        case 5: return {(const void*)prompt_attn_kernel<DT, 5, 16>, 16};
-        case 6: return {(const void*)prompt_attn_kernel<DT, 6, 16>, 16};
+        case 5: return {(const void*)prompt_attn_kernel<DT, 5, 12>, 12};
+        case 6: return {(const void*)prompt_attn_kernel<DT, 6, 12>, 12};
         case 7: return {(const void*)prompt_attn_kernel<DT, 7, 16>, 16};
         case 8: return {(const void*)prompt_attn_kernel<DT, 8, 16>, 16};
         case 9: case 10: case 11: case 12: return {(const void*)prompt_attn_kernel<DT, 12, 32>, 32};
