@@ -25,6 +25,11 @@
 // loads under way, and meet in LDS.  A unit cut by a border is joined from fp32 partials, at most two a
 // workgroup, by the last of its workgroups to arrive (or a second launch), in a fixed order.  Units of few blocks are not
 // cut: the workgroup that has their first block takes them whole.
+//
+// Bound: the cache's bytes, 4352 a block at D = 128 (64 sequences of 1024..8192 tokens, 8 kv heads, bf16: 245 MB in 56.5 us,
+// 4.3 TB/s of the 4.9 a large copy reaches); about 290 vector instructions a block fill a third of the issue slots.  Short
+// calls are latencies: 32 heads of one sequence of 77 tokens 5.9 us.  An even cut against a fixed number of splits a
+// sequence, 32 sequences of 64..4096 tokens: 36.4 us against 45.4.
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
 
@@ -355,250 +360,250 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
     int x = group * R.piece;
     const int end = min(x + R.piece, R.total);
     for (; x < end; __syncthreads()) {
-    const Unit U = unit_at(A, R, x, lane);
-    const bool small = U.blocks <= R.whole;
-    const int from = max(x - U.start, 0), upto = small ? U.blocks : min(U.blocks, end - U.start);
-    // a small unit that starts before the piece is another workgroup's, and so is one whose blocks start behind it
-    const bool mine = small ? x == U.start - A.unit_cost : upto > 0;
-    x = U.start + max(upto, 0);
-    if (!mine) continue;
-    const int part_slot = 2 * group + (from == 0 && U.start != group * R.piece ? 1 : 0);
-    const int b = U.b, h = U.j / A.tiles, tile = U.j - h * A.tiles;
-    const int len = index_at(C.lens, b);
-    const int first = from, last = len > 0 && C.num_pages > 0 ? upto : 0;
+        const Unit U = unit_at(A, R, x, lane);
+        const bool small = U.blocks <= R.whole;
+        const int from = max(x - U.start, 0), upto = small ? U.blocks : min(U.blocks, end - U.start);
+        // a small unit that starts before the piece is another workgroup's, and so is one whose blocks start behind it
+        const bool mine = small ? x == U.start - A.unit_cost : upto > 0;
+        x = U.start + max(upto, 0);
+        if (!mine) continue;
+        const int part_slot = 2 * group + (from == 0 && U.start != group * R.piece ? 1 : 0);
+        const int b = U.b, h = U.j / A.tiles, tile = U.j - h * A.tiles;
+        const int len = index_at(C.lens, b);
+        const int first = from, last = len > 0 && C.num_pages > 0 ? upto : 0;
 
-    // The wave's blocks in turn.  A block without a page counts as unseen; its loads (and those past the last block) go
-    // to the pool's first block, so that the loads under way are always as many and a step waits for its own alone.
-    Block<NS, EXACT> B;
-    auto where = [&](int blk, bool& there) {
-        const uint32_t* p = blk < last ? kv4_block(C, b, blk, h) : nullptr;
-        there = p != nullptr;
-        return there ? p : C.pages;
-    };
-    int blk = first + wave;
-    bool there = false;
-    if (blk < last) {
-        const uint32_t* p = where(blk, there);
-        B.load_k(p, lane);
-        B.load_v(p, lane);
-    }
-
-    // this lane's query row; its newest visible token
-    const int row = 16 * tile + n;
-    const int tok = (int)fdiv((uint32_t)row, A.div_group);
-    const bool real = row < A.rows;
-    const int newest = real ? len - A.t + tok : -1;
-    const int all_see = len - A.t + (int)fdiv((uint32_t)(16 * tile), A.div_group);    // every row sees tokens up to here
-
-    // q scaled to below 2^11, and its sum
-    Op q[TERMS][NS];
-    float cc, cl = 0.f, qsum = 0.f;
-    {
-        float x[NS][8];
-        float top = 0.f;
-        // loads of a row and values that exist, whatever the lane's own, so that all go out at once
-        const long at = out_at<DT>(A, b, h, min(row, A.rows - 1));
-#pragma unroll
-        for (int s = 0; s < NS; ++s) load8<DT>(A.q, at + min(8 * (g * NS + s), D - 8), x[s]);
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const bool has = real && 8 * (g * NS + s) < D;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[s][j] = has ? x[s][j] : 0.f;
-                top = fmaxf(top, __builtin_fabsf(x[s][j]));
-            }
+        // The wave's blocks in turn.  A block without a page counts as unseen; its loads (and those past the last block) go
+        // to the pool's first block, so that the loads under way are always as many and a step waits for its own alone.
+        Block<NS, EXACT> B;
+        auto where = [&](int blk, bool& there) {
+            const uint32_t* p = blk < last ? kv4_block(C, b, blk, h) : nullptr;
+            there = p != nullptr;
+            return there ? p : C.pages;
+        };
+        int blk = first + wave;
+        bool there = false;
+        if (blk < last) {
+            const uint32_t* p = where(blk, there);
+            B.load_k(p, lane);
+            B.load_v(p, lane);
         }
-        top = group_max(top);
-        const int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;   // top < 2^e
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = __builtin_ldexpf(x[s][j], 11 - e);
-                const float u = !EXACT && (j & 2) ? v * 0.0625f : v;
-                const _Float16 hi = (_Float16)u;
-                q[0][s].h[j] = hi;
-                float held = (float)hi;
-                if constexpr (TERMS == 2) {
-                    const _Float16 lo = (_Float16)(u - held);
-                    q[1][s].h[j] = lo;
-                    held += (float)lo;
-                }
-                if constexpr (!EXACT) qsum += (j & 2) ? held * 16.f : held;
-            }
-        if constexpr (!EXACT) qsum = group_sum(qsum) * 0x1p-22f;
-        // scale log2 e; for fp32 in two terms: its rounding would bend every score by 2^-24 of itself
-        const double c2 = (double)A.scale * 1.44269504088896340736;
-        cc = __builtin_ldexpf((float)c2, UP - 11 + e);
-        if constexpr (EXACT) cl = __builtin_ldexpf((float)(c2 - (double)(float)c2), UP - 11 + e);
-    }
 
-    f4 acc[TILES], accz = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
-    float M = LOW, la = 0.f, lb = 0.f;
+        // this lane's query row; its newest visible token
+        const int row = 16 * tile + n;
+        const int tok = (int)fdiv((uint32_t)row, A.div_group);
+        const bool real = row < A.rows;
+        const int newest = real ? len - A.t + tok : -1;
+        const int all_see = len - A.t + (int)fdiv((uint32_t)(16 * tile), A.div_group);    // every row sees tokens up to here
 
-    while (blk < last) {
-        bool next_there;
-        const uint32_t* next = where(blk + WAVES, next_there);
-        // scores of 8 tokens: y = s (dot - z sum q), and log2 of the probability's factor = cc y
-        float y[8], sv[8];
+        // q scaled to below 2^11, and its sum
+        Op q[TERMS][NS];
+        float cc, cl = 0.f, qsum = 0.f;
+        {
+            float x[NS][8];
+            float top = 0.f;
+            // loads of a row and values that exist, whatever the lane's own, so that all go out at once
+            const long at = out_at<DT>(A, b, h, min(row, A.rows - 1));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            f4 s = {0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < NS; ++s) load8<DT>(A.q, at + min(8 * (g * NS + s), D - 8), x[s]);
 #pragma unroll
-            for (int st = 0; st < NS; ++st) {
-                if constexpr (EXACT) {
-                    const _Float16 z = (_Float16)(float)(B.kz[i] & 15u);
-                    const h2 lo = h2{(_Float16)-256.f, (_Float16)-256.f} - h2{z, z};
-                    const h2 hi = h2{(_Float16)-16.f, (_Float16)-16.f} - h2{z, z};
-                    const h8 kc = decode_exact(B.k[i][st], lo, hi, lo, hi);
-                    s = mfma(kc, q[0][st].v, s);
-                    s = mfma(kc, q[1][st].v, s);
-                } else {
-                    s = mfma(decode(B.k[i][st]), q[0][st].v, s);
+            for (int s = 0; s < NS; ++s) {
+                const bool has = real && 8 * (g * NS + s) < D;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[s][j] = has ? x[s][j] : 0.f;
+                    top = fmaxf(top, __builtin_fabsf(x[s][j]));
                 }
             }
+            top = group_max(top);
+            const int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;   // top < 2^e
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w = B.km[i][j];
-                y[4 * i + j] = __uint_as_float(w) * (EXACT ? s[j] : __builtin_fmaf(-(float)(w & 15u), qsum, s[j]));
-            }
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = __builtin_ldexpf(x[s][j], 11 - e);
+                    const float u = !EXACT && (j & 2) ? v * 0.0625f : v;
+                    const _Float16 hi = (_Float16)u;
+                    q[0][s].h[j] = hi;
+                    float held = (float)hi;
+                    if constexpr (TERMS == 2) {
+                        const _Float16 lo = (_Float16)(u - held);
+                        q[1][s].h[j] = lo;
+                        held += (float)lo;
+                    }
+                    if constexpr (!EXACT) qsum += (j & 2) ? held * 16.f : held;
+                }
+            if constexpr (!EXACT) qsum = group_sum(qsum) * 0x1p-22f;
+            // scale log2 e; for fp32 in two terms: its rounding would bend every score by 2^-24 of itself
+            const double c2 = (double)A.scale * 1.44269504088896340736;
+            cc = __builtin_ldexpf((float)c2, UP - 11 + e);
+            if constexpr (EXACT) cl = __builtin_ldexpf((float)(c2 - (double)(float)c2), UP - 11 + e);
         }
-        // the next block's keys, under way from here on (kept behind the last use of this one's, in its registers)
-        __builtin_amdgcn_sched_barrier(0);
-        B.load_k(next, lane);
-        __builtin_amdgcn_sched_barrier(0);
+
+        f4 acc[TILES], accz = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sv[j] = __uint_as_float(B.vm[j >> 2][j & 3]);
-        if (!there || 32 * blk + 31 > all_see) {
-            const int base = there ? 32 * blk + 4 * g : INT32_MAX / 2;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool seen = base + (j & 3) + 16 * (j >> 2) <= newest;
-                y[j] = seen ? y[j] : -__builtin_inff();
-                sv[j] = seen ? sv[j] : 0.f;
-            }
-        }
-        float ym = y[0], sm = sv[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) ym = fmaxf(ym, y[j]), sm = fmaxf(sm, sv[j]);
-        // score + log2 s' is below this for every token of the lane
-        float bound = ym * cc + (float)max(__builtin_amdgcn_frexp_expf(sm), -90);
-        bound = group_max(bound);
-        if (__builtin_amdgcn_ballot_w64(bound > M + SLACK) != 0) {
-            const float to = bound > M + SLACK ? __builtin_ceilf(bound) : M;     // whole: what it scales stays exact
-            const float f = __builtin_amdgcn_exp2f(M - to);
-            M = to;
-            la *= f, lb *= f;
-#pragma unroll
-            for (int i = 0; i < TILES; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] *= f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) accz[j] *= f;
-        }
-        const float ma = HEADROOM - M, mb = EXACT ? ma : HEADROOM - 4.f - M;
-        float w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float at = (j & 2) ? mb : ma;
-            if constexpr (EXACT) at = y[j] > -__builtin_inff() ? __builtin_fmaf(y[j], cl, at) : at;
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, at));
-            if (j & 2) lb += p;
-            else la += p;
-            w[j] = p * sv[j];
-        }
-        Op wo[TERMS], zo;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            wo[0].h[j] = (_Float16)w[j];
-            if constexpr (TERMS == 2) wo[1].h[j] = (_Float16)(w[j] - (float)wo[0].h[j]);
-        }
-        if constexpr (EXACT) {
-            h2 bias[4];                                // of tokens (0, 1), (2, 3), (4, 5), (6, 7)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const h2 z = {(_Float16)(float)(B.vm[i >> 1][2 * (i & 1)] & 15u),
-                              (_Float16)(float)(B.vm[i >> 1][2 * (i & 1) + 1] & 15u)};
-                const _Float16 lead = (_Float16)(i & 1 ? -16.f : -256.f);
-                bias[i] = h2{lead, lead} - z;
-            }
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                const h8 vc = decode_exact(B.v[i], bias[0], bias[1], bias[2], bias[3]);
-                acc[i] = mfma(vc, wo[0].v, acc[i]);
-                acc[i] = mfma(vc, wo[1].v, acc[i]);
-            }
-        } else {
-            // zero points as codes: pairs (0,1), (4,5) plain, (2,3), (6,7) 16-fold
+        for (int i = 0; i < TILES; ++i) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+        float M = LOW, la = 0.f, lb = 0.f;
+
+        while (blk < last) {
+            bool next_there;
+            const uint32_t* next = where(blk + WAVES, next_there);
+            // scores of 8 tokens: y = s (dot - z sum q), and log2 of the probability's factor = cc y
+            float y[8], sv[8];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                zo.u[2 * i] = (__builtin_amdgcn_perm(B.vm[i][1], B.vm[i][0], 0x0C040C00u) & 0x000F000Fu) << 2;
-                zo.u[2 * i + 1] = (__builtin_amdgcn_perm(B.vm[i][3], B.vm[i][2], 0x0C040C00u) & 0x000F000Fu) << 6;
-            }
-            accz = mfma(zo.v, wo[0].v, accz);
+                f4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) acc[i] = mfma(decode(B.v[i]), wo[0].v, acc[i]);
+                for (int st = 0; st < NS; ++st) {
+                    if constexpr (EXACT) {
+                        const _Float16 z = (_Float16)(float)(B.kz[i] & 15u);
+                        const h2 lo = h2{(_Float16)-256.f, (_Float16)-256.f} - h2{z, z};
+                        const h2 hi = h2{(_Float16)-16.f, (_Float16)-16.f} - h2{z, z};
+                        const h8 kc = decode_exact(B.k[i][st], lo, hi, lo, hi);
+                        s = mfma(kc, q[0][st].v, s);
+                        s = mfma(kc, q[1][st].v, s);
+                    } else {
+                        s = mfma(decode(B.k[i][st]), q[0][st].v, s);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = B.km[i][j];
+                    y[4 * i + j] = __uint_as_float(w) * (EXACT ? s[j] : __builtin_fmaf(-(float)(w & 15u), qsum, s[j]));
+                }
+            }
+            // the next block's keys, under way from here on (kept behind the last use of this one's, in its registers)
+            __builtin_amdgcn_sched_barrier(0);
+            B.load_k(next, lane);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sv[j] = __uint_as_float(B.vm[j >> 2][j & 3]);
+            if (!there || 32 * blk + 31 > all_see) {
+                const int base = there ? 32 * blk + 4 * g : INT32_MAX / 2;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool seen = base + (j & 3) + 16 * (j >> 2) <= newest;
+                    y[j] = seen ? y[j] : -__builtin_inff();
+                    sv[j] = seen ? sv[j] : 0.f;
+                }
+            }
+            float ym = y[0], sm = sv[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) ym = fmaxf(ym, y[j]), sm = fmaxf(sm, sv[j]);
+            // score + log2 s' is below this for every token of the lane
+            float bound = ym * cc + (float)max(__builtin_amdgcn_frexp_expf(sm), -90);
+            bound = group_max(bound);
+            if (__builtin_amdgcn_ballot_w64(bound > M + SLACK) != 0) {
+                const float to = bound > M + SLACK ? __builtin_ceilf(bound) : M;     // whole: what it scales stays exact
+                const float f = __builtin_amdgcn_exp2f(M - to);
+                M = to;
+                la *= f, lb *= f;
+#pragma unroll
+                for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) accz[j] *= f;
+            }
+            const float ma = HEADROOM - M, mb = EXACT ? ma : HEADROOM - 4.f - M;
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float at = (j & 2) ? mb : ma;
+                if constexpr (EXACT) at = y[j] > -__builtin_inff() ? __builtin_fmaf(y[j], cl, at) : at;
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, at));
+                if (j & 2) lb += p;
+                else la += p;
+                w[j] = p * sv[j];
+            }
+            Op wo[TERMS], zo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                wo[0].h[j] = (_Float16)w[j];
+                if constexpr (TERMS == 2) wo[1].h[j] = (_Float16)(w[j] - (float)wo[0].h[j]);
+            }
+            if constexpr (EXACT) {
+                h2 bias[4];                                // of tokens (0, 1), (2, 3), (4, 5), (6, 7)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const h2 z = {(_Float16)(float)(B.vm[i >> 1][2 * (i & 1)] & 15u),
+                                  (_Float16)(float)(B.vm[i >> 1][2 * (i & 1) + 1] & 15u)};
+                    const _Float16 lead = (_Float16)(i & 1 ? -16.f : -256.f);
+                    bias[i] = h2{lead, lead} - z;
+                }
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    const h8 vc = decode_exact(B.v[i], bias[0], bias[1], bias[2], bias[3]);
+                    acc[i] = mfma(vc, wo[0].v, acc[i]);
+                    acc[i] = mfma(vc, wo[1].v, acc[i]);
+                }
+            } else {
+                // zero points as codes: pairs (0,1), (4,5) plain, (2,3), (6,7) 16-fold
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    zo.u[2 * i] = (__builtin_amdgcn_perm(B.vm[i][1], B.vm[i][0], 0x0C040C00u) & 0x000F000Fu) << 2;
+                    zo.u[2 * i + 1] = (__builtin_amdgcn_perm(B.vm[i][3], B.vm[i][2], 0x0C040C00u) & 0x000F000Fu) << 6;
+                }
+                accz = mfma(zo.v, wo[0].v, accz);
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) acc[i] = mfma(decode(B.v[i]), wo[0].v, acc[i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            B.load_v(next, lane);
+            blk += WAVES;
+            there = next_there;
         }
-        __builtin_amdgcn_sched_barrier(0);
-        B.load_v(next, lane);
-        blk += WAVES;
-        there = next_there;
-    }
 
-    // the waves' rows meet
-    float l = group_sum(EXACT ? la + lb : __builtin_fmaf(16.f, lb, la));
-    if (g == 0) red_m[wave][n] = M, red_l[wave][n] = l;
-    __syncthreads();
-    float top = red_m[0][n];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, red_m[w][n]);
-    const float f = __builtin_amdgcn_exp2f(M - top) * (EXACT ? 1.f : 0x1p22f);
-#pragma unroll
-    for (int turn = 0; turn < 2; ++turn) {             // waves 0 and 1 write, 2 and 3 add
-        if ((wave >> 1) == turn) {
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                float4* at = reinterpret_cast<float4*>(&red[wave & 1][n][16 * i + 4 * g]);
-                float4 o = turn ? *at : float4{0.f, 0.f, 0.f, 0.f};
-                o.x += (acc[i][0] - accz[0]) * f, o.y += (acc[i][1] - accz[0]) * f;
-                o.z += (acc[i][2] - accz[0]) * f, o.w += (acc[i][3] - accz[0]) * f;
-                *at = o;
-            }
-        }
+        // the waves' rows meet
+        float l = group_sum(EXACT ? la + lb : __builtin_fmaf(16.f, lb, la));
+        if (g == 0) red_m[wave][n] = M, red_l[wave][n] = l;
         __syncthreads();
-    }
-    const bool all = from == 0 && upto == U.blocks;
-    const int cols = min(16, A.rows - 16 * tile);
-    for (int y = threadIdx.x; y < cols * (D >> 2); y += 64 * WAVES) {
-        const int c = y / (D >> 2), d = (y - c * (D >> 2)) * 4;
-        float o[4], ls = 0.f, mt = red_m[0][c];
+        float top = red_m[0][n];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) mt = fmaxf(mt, red_m[w][c]);
+        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, red_m[w][n]);
+        const float f = __builtin_amdgcn_exp2f(M - top) * (EXACT ? 1.f : 0x1p22f);
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) ls += red_l[w][c] * __builtin_amdgcn_exp2f(red_m[w][c] - mt);
+        for (int turn = 0; turn < 2; ++turn) {             // waves 0 and 1 write, 2 and 3 add
+            if ((wave >> 1) == turn) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = red[0][c][d + i] + red[1][c][d + i];
-        if (all) {
-            const float inv = ls == 0.f ? 0.f : 1.f / ls;
-            const long at = out_at<DT>(A, b, h, 16 * tile + c) + d;
+                for (int i = 0; i < TILES; ++i) {
+                    float4* at = reinterpret_cast<float4*>(&red[wave & 1][n][16 * i + 4 * g]);
+                    float4 o = turn ? *at : float4{0.f, 0.f, 0.f, 0.f};
+                    o.x += (acc[i][0] - accz[0]) * f, o.y += (acc[i][1] - accz[0]) * f;
+                    o.z += (acc[i][2] - accz[0]) * f, o.w += (acc[i][3] - accz[0]) * f;
+                    *at = o;
+                }
+            }
+            __syncthreads();
+        }
+        const bool all = from == 0 && upto == U.blocks;
+        const int cols = min(16, A.rows - 16 * tile);
+        for (int y = threadIdx.x; y < cols * (D >> 2); y += 64 * WAVES) {
+            const int c = y / (D >> 2), d = (y - c * (D >> 2)) * 4;
+            float o[4], ls = 0.f, mt = red_m[0][c];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) store_f<DT>(A.out, at + i, o[i] * inv);
-        } else {
-            const __amdgpu_buffer_rsrc_t buf = buffer_of(part_sums(A, part_slot), (long)A.cols * D);
-            const u4 v = {__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])};
-            __builtin_amdgcn_raw_buffer_store_b128(v, buf, (c * D + d) * 4, 0, SC1);
-            if (d == 0) {
-                float* r = part_rows(A, part_slot) + 2 * c;
-                partial_put(r, mt), partial_put(r + 1, ls);
+            for (int w = 1; w < WAVES; ++w) mt = fmaxf(mt, red_m[w][c]);
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) ls += red_l[w][c] * __builtin_amdgcn_exp2f(red_m[w][c] - mt);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = red[0][c][d + i] + red[1][c][d + i];
+            if (all) {
+                const float inv = ls == 0.f ? 0.f : 1.f / ls;
+                const long at = out_at<DT>(A, b, h, 16 * tile + c) + d;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) store_f<DT>(A.out, at + i, o[i] * inv);
+            } else {
+                const __amdgpu_buffer_rsrc_t buf = buffer_of(part_sums(A, part_slot), (long)A.cols * D);
+                const u4 v = {__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])};
+                __builtin_amdgcn_raw_buffer_store_b128(v, buf, (c * D + d) * 4, 0, SC1);
+                if (d == 0) {
+                    float* r = part_rows(A, part_slot) + 2 * c;
+                    partial_put(r, mt), partial_put(r + 1, ls);
+                }
             }
         }
-    }
-    if (all || !A.split_cnt) continue;
-    const Parts P = parts_of(R, U);
-    if (split_arrive(A.split_cnt + P.first, P.count, &flag)) combine<DT>(A, lds.combine, P, b, h, tile);
+        if (all || !A.split_cnt) continue;
+        const Parts P = parts_of(R, U);
+        if (split_arrive(A.split_cnt + P.first, P.count, &flag)) combine<DT>(A, lds.combine, P, b, h, tile);
     }
 }
 

@@ -3,7 +3,8 @@
 // prompt_attn.hip's arithmetic with nothing rounded below fp32: S^T = K q^T and O^T += V^T w on
 // v_mfma_f32_32x32x2_f32, whose S^T layout (column = row, tokens 8 i + 4 (lane / 32) + 0..3) again gives the
 // operand of w without moving it: step i of the second product takes the two tokens that lanes l and l + 32
-// hold in register i.  A workgroup has 64 rows of one head (32 a wave); tiles of 32 tokens pass through LDS.
+// hold in register i.  A workgroup has 64 rows of one head (32 a wave); tiles of 32 tokens pass through LDS.  Bound: the fp32
+// matrix instructions, a sixteenth of the 16-bit rate, and the tile's staging, which nothing hides.
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
 

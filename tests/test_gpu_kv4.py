@@ -225,6 +225,25 @@ def test_attention_long_and_split(hip):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_many_sequences(hip, dtype):
+    """More sequences than a wave looks at at once, empty ones and long ones among them: units whole, cut once and cut often."""
+    lens = [(7 * i) % 45 for i in range(150)]
+    lens[3], lens[70], lens[149] = 1500, 700, 900
+    cache, pages, table, ln = _case(lens, 1, 64, 32, 40, dtype)
+    q = torch.randn(150, 2, 64, generator=torch.Generator().manual_seed(41)).to(dtype)
+    got = _check(q, cache, pages, table, ln)
+    assert not got[0].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_row_tiles_cut(hip, dtype):
+    """Several tiles of query rows a head, the last one part full, over sequences long enough to be cut."""
+    cache, pages, table, ln = _case([2100, 50, 640], 2, 128, 64, 42, dtype)
+    q = torch.randn(3, 9, 8, 128, generator=torch.Generator().manual_seed(43)).to(dtype)
+    _check(q, cache, pages, table, ln)
+
+
 def test_attention_scales_and_magnitudes(hip):
     """Sharp and flat softmax, scales of tokens spread over orders of magnitude, tiny and huge values."""
     for spread, size, scale in ((0.1, 1.0, 3.0), (3.0, 1.0, 0.02), (1.0, 1e-6, 1e5), (1.0, 1e4, 1e-7)):
