@@ -371,6 +371,13 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// Barrier behind which every wave's loads into LDS have landed.  They count as vector memory: a wave has to wait for its
+// own before the barrier, and __syncthreads does not promise that wait.
+__device__ __forceinline__ void landed_barrier() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // ---------------------------------------------------------------- scalar code access
 // Code j (0..31) of a chunk held in BITS registers (straddling codes of W3 are
 // joined with a 64-bit funnel shift).

@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
     // Every turn has one barrier, so that waves may be in different loops.
     bool again = false;
     auto turn = [&](int t) {
-        __syncthreads();                                          // tile t has landed; tile t - 1 has been read
+        landed_barrier();                                         // tile t has landed; tile t - 1 has been read
         if (t + 1 < tiles) stage(t + 1, (t + 1) & 1);
     };
     for (int t0 = 0;;) {
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
         }
         for (; t < tiles; ++t) {
             if (again) {
-                __syncthreads();
+                landed_barrier();
                 for (int x = threadIdx.x; x < KT * CP; x += 64 * WAVES) {
                     u4* at = reinterpret_cast<u4*>(lds + (2 * (t & 1) + 1) * TILE) + x;
                     u4 v = *at;
