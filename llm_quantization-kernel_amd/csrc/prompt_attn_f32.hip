@@ -3,8 +3,14 @@
 // prompt_attn.hip's arithmetic with nothing rounded below fp32: S^T = K q^T and O^T += V^T w on
 // v_mfma_f32_32x32x2_f32, whose S^T layout (column = row, tokens 8 i + 4 (lane / 32) + 0..3) again gives the
 // operand of w without moving it: step i of the second product takes the two tokens that lanes l and l + 32
-// hold in register i.  A workgroup has 64 rows of one head (32 a wave); tiles of 32 tokens pass through LDS.  Bound: the fp32
-// matrix instructions, a sixteenth of the 16-bit rate, and the tile's staging, which nothing hides.
+// hold in register i.  A workgroup has 128 rows of one head (32 a wave); tiles of 32 tokens are staged in LDS as in
+// prompt_attn.hip, the next one's loads under way.  The order of a product's steps is free: lanes l and l + 32 take four
+// neighbouring values each, so that K comes in 16-byte reads.
+// Bound: the fp32 matrix instructions, a sixteenth of the 16-bit rate, each waiting for the one before: a tile is one chain
+// of D / 2 products and D / 32 of sixteen, and one or two waves share a SIMD.  Measured: 1024 rows, 32 heads of 128, 255 us
+// (34 TFLOP/s; with loads through registers and two waves a workgroup 561); 4 x 100..700 rows, 16 / 4 heads of 80, 131 us
+// (216).  The scores in two sums instead of one: 260 and 129.  1500 rows, 8 heads of 256: 750 us (2143), 96 workgroups on
+// 256 CUs, the last with 47 tiles in a row.
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
 
@@ -13,19 +19,37 @@ namespace {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-constexpr int WAVES = 2;
+constexpr int WAVES = 4;
 constexpr int ROWS = 32 * WAVES;
 constexpr int KT = 32;
 constexpr float LOW = -1e30f;
 
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(3))) f4* lds_f4;
+typedef const __attribute__((address_space(3))) float* lds_f1;
+
+// The chunk of K's row r that lies at chunk c (and the other way round): a wave reads two neighbouring chunks of 32 rows.
+template <int CP>
+__device__ __forceinline__ int k_turn(int r, int c) { return c ^ (CP % 16 == 0 ? (r & 7) << 1 : (r >> 1 & 3) << 1); }
+
+// A buffer over a sequence's rows (len of them, `stride` elements apart, D values each) from tile t on.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float* base, long stride, int t, int len, int D) {
+    const long left = len - t * KT;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + (long)t * KT * stride), 0,
+                                             (int)min(((left - 1) * stride + D) * 4, 0x7FFFFF00l), 0x00020000);
+}
+
+__device__ __forceinline__ void load_chunks(__amdgpu_buffer_rsrc_t from, uint32_t to, uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)to, 16, offset, 0, 0, 0);
+}
+
 // DP: the head's values rounded up to 32 (64 above 128).
 template <int DP>
 __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptArgs A, int row_tiles) {
-    constexpr int DT32 = DP / 32;
-    constexpr int PITCH = DP + 1;                      // odd: a wave reads 32 rows' values of one column
-    extern __shared__ __align__(16) float lds_f[];     // K tile [KT][PITCH], V tile [KT][DP]
-    float* kt = lds_f;
-    float* vt = lds_f + KT * PITCH;
+    constexpr int DT32 = DP / 32, CP = DP / 4;         // d tiles, 16-byte chunks of a row
+    constexpr int TILE = KT * CP * 16;                 // bytes of a K or V tile
+    extern __shared__ __align__(16) char lds[];        // [2][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hf = lane >> 5;
     int id = blockIdx.x;
@@ -55,12 +79,33 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
     const float* vp = reinterpret_cast<const float*>(A.v) + (long)start * A.v_row + hk * A.v_head;
     const int wq = q0 + 32 * wave, row = wq + n;
 
-    float q[DP / 2];                                   // values 2 s + hf
+    f4 q[DP / 8];                                      // values 8 u + 4 hf ..
     {
         const float* qp = reinterpret_cast<const float*>(A.q) + (long)(start + min(row, len - 1)) * A.q_row + h * A.q_head;
 #pragma unroll
-        for (int s = 0; s < DP / 2; ++s) q[s] = 2 * s + hf < D ? qp[2 * s + hf] : 0.f;
+        for (int u = 0; u < DP / 8; ++u) {
+            const int d = 8 * u + 4 * hf;
+            q[u] = d < D ? *reinterpret_cast<const f4*>(qp + d) : f4{0.f, 0.f, 0.f, 0.f};
+        }
     }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)lds;
+    constexpr int LOADS = KT * CP / (64 * WAVES);      // a lane's loads of a tile, and where its chunks come from
+    uint32_t k_off[LOADS], v_off[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int pos = (i * WAVES + wave) * 64 + lane, r = pos / CP, c = pos % CP, ck = k_turn<CP>(r, c);
+        k_off[i] = 4 * ck < D ? r * (uint32_t)A.k_row * 4 + 16 * ck : 0x7FFFFFF0u;
+        v_off[i] = 4 * c < D ? r * (uint32_t)A.v_row * 4 + 16 * c : 0x7FFFFFF0u;
+    }
+    auto stage = [&](int t) {
+        const __amdgpu_buffer_rsrc_t kr = rows_from(kp, A.k_row, t, len, D), vr = rows_from(vp, A.v_row, t, len, D);
+        const uint32_t to = lds0 + (t & 1) * 2 * TILE + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            load_chunks(kr, to + i * WAVES * 1024, k_off[i]);
+            load_chunks(vr, to + TILE + i * WAVES * 1024, v_off[i]);
+        }
+    };
     f16v acc[DT32];
 #pragma unroll
     for (int i = 0; i < DT32; ++i)
@@ -72,23 +117,23 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
     const float cc = (float)c2, cl = (float)(c2 - (double)cc);
     bool odd_values = false;
 
-    const int last = min(q0 + ROWS, len);
-    for (int t0 = 0; t0 < last; t0 += KT) {
-        __syncthreads();
-        for (int x = threadIdx.x; x < KT * DP; x += 64 * WAVES) {
-            const int r = x / DP, d = x % DP;
-            const long tok = min(t0 + r, len - 1);
-            kt[r * PITCH + d] = d < D ? kp[tok * A.k_row + d] : 0.f;
-            vt[x] = d < D ? vp[tok * A.v_row + d] : 0.f;
-        }
-        __syncthreads();
+    const int tiles = (min(q0 + ROWS, len) + KT - 1) / KT;
+    stage(0);
+    for (int t = 0; t < tiles; ++t) {
+        landed_barrier();                              // tile t has landed; tile t - 1 has been read
+        if (t + 1 < tiles) stage(t + 1);
+        const int t0 = t * KT;
         if (t0 > wq + 31) continue;
+        const uint32_t kt = lds0 + (t & 1) * 2 * TILE, vt = kt + TILE;
         f16v s;
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = 0.f;
 #pragma unroll
-        for (int st = 0; st < DP / 2; ++st)
-            s = __builtin_amdgcn_mfma_f32_32x32x2f32(kt[n * PITCH + 2 * st + hf], q[st], s, 0, 0, 0);
+        for (int u = 0; u < DP / 8; ++u) {
+            const f4 k = *reinterpret_cast<lds_f4>(kt + 16 * (n * CP + k_turn<CP>(n, 2 * u + hf)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[u][e], s, 0, 0, 0);
+        }
         const bool edge = t0 + KT - 1 > wq;
         float top = -__builtin_inff();
 #pragma unroll
@@ -119,7 +164,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
         for (int i = 0; i < DT32; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                float v = vt[(8 * (j >> 2) + 4 * hf + (j & 3)) * DP + 32 * i + n];
+                float v = *reinterpret_cast<lds_f1>(vt + ((8 * (j >> 2) + 4 * hf + (j & 3)) * DP + 32 * i + n) * 4);
                 if (edge && !(__builtin_fabsf(v) < __builtin_inff())) v = 0.f, odd_values = true;
                 acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[j], acc[i], 0, 0, 0);
             }
@@ -149,7 +194,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
 
 template <int DP>
 const void* built(int& lds) {
-    lds = (KT * (DP + 1) + KT * DP) * 4;
+    lds = 4 * KT * DP * 4;
     return (const void*)prompt_attn_f32_kernel<DP>;
 }
 
