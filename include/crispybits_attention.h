@@ -48,7 +48,7 @@ int cbk_kv4_append(int32_t* pages, int64_t num_pages, int64_t kv_heads, int head
                    const int32_t* cu_seqlens, int64_t num_seqs, int device, void* stream);
 
 /* The reverse: the values that the same rows are held as, into contiguous k and v [rows, kv_heads, head_dim].
- * Tokens that are not stored and rows of no sequence come back as zeros. */
+ * Tokens that are not stored and rows of no sequence come back as zeros.  At most 2^28 rows, as above. */
 int cbk_kv4_read(const int32_t* pages, int64_t num_pages, int64_t kv_heads, int head_dim, int64_t page_size,
                  void* k, void* v, int dtype, int64_t rows,
                  const int32_t* block_table, int64_t table_width, const int32_t* seq_lens,
@@ -67,7 +67,8 @@ int cbk_kv4_attention(const void* q, int dtype, int64_t num_seqs, int64_t t, int
 
 /* Causal attention over packed prompts: row i of sequence b attends to rows 0 .. i of it.  q [rows, heads,
  * head_dim], k and v [rows, kv_heads, head_dim] with strides, out contiguous [rows, heads, head_dim].  max_seqlen
- * (0 < max_seqlen <= rows) bounds every sequence's length; rows of a longer one past it are not computed.  Rows of no
+ * (0 < max_seqlen <= rows) bounds every sequence's length; rows of a longer one past it are not computed;
+ * ceil(max_seqlen / 128) (num_seqs + 1) heads must be below 2^24.  Rows of no
  * sequence (behind the last) are set to zero when zero_tail, else left as they were.  Places that the mask
  * hides take no part whatever they hold.  scale > 0. */
 int cbk_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t rows, int64_t heads,

@@ -17,6 +17,8 @@ namespace {
 constexpr int64_t MOST = INT32_MAX / 2;        // rows, pages, tokens of a table: positions stay in 32 bits
 constexpr int64_t MOST_GRID = 65535;           // the second and third grid dimension
 
+constexpr int64_t MOST_GROUPS = (1 << 24) - 1; // workgroups of 256 threads: a launch has fewer than 2^32 threads
+constexpr int64_t MOST_STORED = 1 << 28;       // rows of an append or a read (32 a workgroup)
 constexpr int64_t MAX_ROW_STRIDE = 1 << 23;
 
 bool valid_dtype(int dt) { return dt == CBK_F16 || dt == CBK_BF16 || dt == CBK_F32; }
@@ -72,7 +74,7 @@ int view(const char* what, const int32_t* pages, int64_t num_pages, int64_t kv_h
 }
 
 int check_rows(const char* what, int64_t rows, const int32_t* cu, int64_t seqs) {
-    if (rows < 0 || rows > MOST) return fail(CBK_EINVAL, "%s: bad number of rows", what);
+    if (rows < 0 || rows > MOST_STORED) return fail(CBK_EINVAL, "%s: bad number of rows", what);
     if (!cu && rows != seqs) return fail(CBK_EINVAL, "%s: without cu_seqlens there is one row a sequence", what);
     return CBK_OK;
 }
@@ -225,7 +227,7 @@ int cbk_prompt_attention(const void* q, const void* k, const void* v, int dtype,
         return fail(CBK_EINVAL, "%s: q, k, v, out and cu_seqlens must be non-null", what);
     if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out))
         return fail(CBK_EINVAL, "%s: q, k, v and out must be 16-byte aligned", what);
-    if ((max_seqlen + 31) / 32 * (num_seqs + 1) * heads > INT32_MAX)
+    if ((max_seqlen + 127) / 128 * (num_seqs + 1) * heads > MOST_GROUPS)
         return fail(CBK_EINVAL, "%s: max_seqlen x sequences x heads is too large", what);
     PromptArgs A = {};
     A.q = q, A.k = k, A.v = v, A.out = out, A.cu = cu_seqlens;

@@ -92,7 +92,7 @@ Pool pool_of(const Tensor& pages, int64_t page_size, int64_t head_dim, const Ten
              const OptT& cu) {
     TORCH_CHECK(pages.is_cuda() && pages.scalar_type() == at::kInt && pages.dim() == 3 && pages.is_contiguous(),
                 "pages must be a contiguous CUDA int32 tensor [pages, kv heads, words]");
-    const int64_t words = cbk_kv4_page_words((int)head_dim, page_size);
+    const int64_t words = head_dim > 0 && head_dim <= 256 ? cbk_kv4_page_words((int)head_dim, page_size) : -1;
     TORCH_CHECK(words > 0, "head_dim must be a multiple of 8 up to 256, page_size a power of two from 32 to 65536");
     TORCH_CHECK(pages.size(2) == words, "pages of ", page_size, " tokens and head_dim ", head_dim, " have ", words,
                 " words, not ", pages.size(2));
@@ -173,6 +173,7 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
     TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
                 "k and v must be [rows, kv heads, head_dim] with q's rows and head_dim");
+    TORCH_CHECK(q.size(2) <= 256, "prompt_attention: head_dim must be a multiple of 8 up to 256");
     const int32_t* c = index_ptr(cu, q, "cu_seqlens", 1);
     TORCH_CHECK(cu.size(0) >= 1, "cu_seqlens must have one more entry than there are sequences");
     const Tensor qr = rows_of(q), kr = rows_of(k), vr = rows_of(v);

@@ -66,7 +66,7 @@ def _append(**kw):
     (dict(kr=-256), "16-byte aligned"), (dict(k=ALIGNED + 8), "16-byte aligned"), (dict(pages=ALIGNED + 4), "16-byte aligned"),
     (dict(table=None), "non-null"), (dict(lens=None), "non-null"), (dict(pages=None), "non-null"), (dict(v=None), "non-null"),
     (dict(cu=None), "one row a sequence"), (dict(rows=-1), "number of rows"), (dict(seqs=70000), "at most"),
-    (dict(width=1 << 30), "too wide"),
+    (dict(width=1 << 30), "too wide"), (dict(rows=(1 << 28) + 1), "number of rows"),
 ])
 def test_append_refusals(kw, msg):
     assert _append(**kw) == 1 and msg in _err()
@@ -91,6 +91,7 @@ def _read(**kw):
 @pytest.mark.parametrize("kw,msg", [
     (dict(dtype=-1), "fp16/bf16/fp32"), (dict(page=33), "page_size must be"), (dict(k=ALIGNED + 2), "16-byte aligned"),
     (dict(k=None), "non-null"), (dict(cu=None), "one row a sequence"), (dict(seqs=0), "rows without a sequence"),
+    (dict(rows=(1 << 28) + 1), "number of rows"),
 ])
 def test_read_refusals(kw, msg):
     assert _read(**kw) == 1 and msg in _err()
@@ -139,6 +140,7 @@ def _prompt(**kw):
     (dict(scale=0.0), "scale must be"), (dict(longest=0), "max_seqlen must be"), (dict(longest=101), "max_seqlen must be"),
     (dict(seqs=0), "rows without a sequence"), (dict(seqs=70000), "at most"), (dict(rows=-5), "number of rows"),
     (dict(rows=1 << 29, longest=1 << 29, heads=4, seqs=1000), "too large"),
+    (dict(rows=1 << 22, longest=1 << 22, heads=4, seqs=128), "too large"),      # 2^15 x 129 x 4 workgroups of 256
 ])
 def test_prompt_refusals(kw, msg):
     assert _prompt(**kw) == 1 and msg in _err()
