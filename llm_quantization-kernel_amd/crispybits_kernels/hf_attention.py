@@ -35,12 +35,12 @@ class KV4Layer(CacheLayerMixin):
     def update(self, key_states, value_states, *args, **kwargs):
         b, heads, s, d = key_states.shape
         o = self.owner
-        if b > o.sequences or self.seen + s > o.tokens:
-            raise ValueError(f"{b} sequences of {self.seen + s} tokens do not fit a cache of {o.sequences} x "
-                             f"{o.tokens}")
-        self.seen += s
+        n = self.seen + s
+        if b > o.sequences or n > o.tokens:
+            raise ValueError(f"{b} sequences of {n} tokens do not fit a cache of {o.sequences} x {o.tokens}")
         k, v = (t.transpose(1, 2).reshape(b * s, heads, d) for t in (key_states, value_states))
-        kv4_append(self.cache, k, v, o.block_table[:b], o.lengths(self.seen)[:b], None if s == 1 else o.starts(b, s))
+        kv4_append(self.cache, k, v, o.block_table[:b], o.lengths(n)[:b], None if s == 1 else o.starts(b, s))
+        self.seen = n
         setattr(key_states, _LAYER, self)
         return key_states, value_states
 
@@ -57,7 +57,7 @@ class KV4Layer(CacheLayerMixin):
         self.seen = 0
 
     def crop(self, tokens_to_remove: int):
-        self.seen = max(0, self.seen - int(tokens_to_remove))
+        self.seen -= min(max(int(tokens_to_remove), 0), self.seen)
 
     def batch_select_indices(self, indices: torch.Tensor):
         """Sequence i becomes sequence indices[i]."""
@@ -97,7 +97,11 @@ class PagedKV4Cache(Cache):
                                                                device)) for _ in range(config.num_hidden_layers)])
 
     def lengths(self, n: int) -> torch.Tensor:
-        """seq_lens, at n: one fill a step, the layers of a step share it."""
+        """seq_lens, at n: one fill a step, the layers of a step share it.  The count is the host's, so a captured step
+        would replay at one length."""
+        if self.seq_lens.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKV4Cache counts tokens on the host: a captured step calls kv4_append and kv4_attention "
+                               "with lengths of its own")
         if self._length != n:
             self.seq_lens.fill_(n)
             self._length = n
@@ -118,7 +122,7 @@ def _mask(batch_size=None, q_length=None, kv_length=None, mask_function=causal_m
     """No mask is made; what the ops cannot do is refused."""
     if mask_function is not causal_mask_function:
         raise ValueError("crispybits attention is plainly causal: no sliding window, packed positions or mask function")
-    if attention_mask is not None and q_length != 1 and not bool(attention_mask.all()):
+    if attention_mask is not None and not bool(attention_mask.all()):
         raise ValueError("crispybits attention takes no padding: give it prompts of one length")
     return None
 

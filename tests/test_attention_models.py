@@ -121,6 +121,26 @@ def test_model_refusals(cpu):
             model(tokens[:, :1], past_key_values=out.past_key_values)
 
 
+def test_masks_and_refused_updates_of_later_steps(cpu):
+    """A mask that hides an earlier token is refused at single tokens too; a refused update and a crop by less than
+    nothing leave the count of tokens as it was."""
+    model = install_attention(_model("llama"))
+    tokens = torch.zeros(2, 6, dtype=torch.long)
+    cache = kv4_cache(model, 2, 8, 32)
+    with torch.no_grad():
+        model(tokens, past_key_values=cache)
+        mask = torch.ones(2, 7, dtype=torch.long)
+        mask[1, 0] = 0
+        with pytest.raises(ValueError, match="no padding"):
+            model(tokens[:, :1], attention_mask=mask, past_key_values=cache)
+        with pytest.raises(ValueError, match="do not fit"):
+            model(tokens[:, :3], past_key_values=cache)
+        cache.crop(-3)
+        assert cache.get_seq_length() == 6
+        model(tokens[:, :1], attention_mask=torch.ones(2, 7, dtype=torch.long), past_key_values=cache)
+        assert cache.get_seq_length() == 7
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,heads,kv,hidden", [("llama", 4, 2, 256), ("llama", 4, 4, 512), ("opt", 4, 4, 320)])
 def test_packed_model(hip, tmp_path, monkeypatch, kind, heads, kv, hidden):
