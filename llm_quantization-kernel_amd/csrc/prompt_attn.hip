@@ -93,9 +93,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const uint16_t* base
                                              (int)min(((left - 1) * stride + D) * 2, 0x7FFFFF00l), 0x00020000);
 }
 
-// 16 bytes a lane from the buffer to LDS, the lanes' behind each other from `to` on.
-__device__ __forceinline__ void load_chunks(__amdgpu_buffer_rsrc_t from, uint32_t to, uint32_t offset, uint32_t rows) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)to, 16, offset, rows, 0, 0);
+// 16 bytes a lane from the buffer to LDS, the lanes' behind each other from `to` on.  All of the offset is the lane's: the
+// range check need not count a scalar offset.
+__device__ __forceinline__ void load_chunks(__amdgpu_buffer_rsrc_t from, uint32_t to, uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)to, 16, offset, 0, 0, 0);
 }
 
 // KS: steps of 16 of the head's values, DT32: tiles of 32, CP: chunks of a row in LDS.
@@ -172,8 +173,8 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
         const uint32_t to = lds0 + buf * 2 * TILE + wave * 1024;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            load_chunks(kr, to + i * WAVES * 1024, k_off[i % PLACES], i * STEP * k_bytes);
-            load_chunks(vr, to + TILE + i * WAVES * 1024, v_off[i % PLACES], i * STEP * v_bytes);
+            load_chunks(kr, to + i * WAVES * 1024, k_off[i % PLACES] + i * STEP * k_bytes);
+            load_chunks(vr, to + TILE + i * WAVES * 1024, v_off[i % PLACES] + i * STEP * v_bytes);
         }
     };
 
