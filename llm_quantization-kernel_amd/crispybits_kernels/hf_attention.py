@@ -57,7 +57,9 @@ class KV4Layer(CacheLayerMixin):
         self.seen = 0
 
     def crop(self, tokens_to_remove: int):
-        self.seen -= min(max(int(tokens_to_remove), 0), self.seen)
+        """-n drops the newest n tokens (rejected drafts); a positive number, the older form, is the length to keep."""
+        n = int(tokens_to_remove)
+        self.seen = min(self.seen, n) if n > 0 else max(self.seen + n, 0)
 
     def batch_select_indices(self, indices: torch.Tensor):
         """Sequence i becomes sequence indices[i]."""

@@ -1,0 +1,74 @@
+"""``PagedKV4Cache`` under the rules that Hugging Face's caches follow, on the CPU oracle in float64: what a crop keeps, and
+generation with drafted tokens that are checked and dropped."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+transformers = pytest.importorskip("transformers")
+
+from transformers.cache_utils import DynamicCache  # noqa: E402
+
+from crispybits_kernels import install_attention, kv4_cache, ops  # noqa: E402
+from oracle import attention as O  # noqa: E402
+from oracle import emulator  # noqa: E402
+
+
+@pytest.fixture(autouse=True)
+def cpu():
+    prev = ops._C
+    both = {n: getattr(emulator, n) for n in dir(emulator) if not n.startswith("_")}
+    both.update({n: getattr(O, n) for n in ("kv4_page_words", "kv4_append", "kv4_read", "kv4_attention", "prompt_attention")})
+    ops.set_backend(SimpleNamespace(**both))
+    yield
+    ops.set_backend(prev)
+
+
+def _llama(**kw):
+    torch.manual_seed(0)
+    cfg = transformers.LlamaConfig(**{**dict(hidden_size=64, intermediate_size=96, num_hidden_layers=2, num_attention_heads=4,
+                                             num_key_value_heads=2, vocab_size=128), **kw})
+    return install_attention(transformers.LlamaForCausalLM(cfg).double().eval())
+
+
+def test_crop_keeps_what_a_dynamic_cache_keeps():
+    """A negative number removes that many tokens, a positive one (the older form) is the length to keep."""
+    model = _llama()
+    tokens = torch.randint(0, 128, (2, 9), generator=torch.Generator().manual_seed(1))
+    for crops in ([-3], [-9], [-20], [0], [4], [9], [30], [-2, 5, -1]):
+        cache, plain = kv4_cache(model, 2, 32, 32), DynamicCache()
+        plain.update(torch.zeros(2, 2, 9, 16), torch.zeros(2, 2, 9, 16), 0)
+        with torch.no_grad():
+            model(tokens, past_key_values=cache)
+            for n in crops:
+                cache.crop(n)
+                plain.crop(n)
+            assert cache.get_seq_length() == plain.get_seq_length(), crops
+            kept = cache.get_seq_length()
+            if kept < 9:                                       # the removed tokens, fed again, are the newest ones
+                again = model(tokens[:, kept:], past_key_values=cache).logits
+                assert cache.get_seq_length() == 9
+                whole = kv4_cache(model, 2, 32, 32)
+                want = [model(t, past_key_values=whole).logits for t in (tokens[:, :kept], tokens[:, kept:]) if t.shape[1]]
+                torch.testing.assert_close(again, want[-1], atol=1e-5, rtol=1e-5)
+
+
+@pytest.mark.parametrize("drafts", [dict(prompt_lookup_num_tokens=4), dict(assistant=True)])
+def test_checked_drafts_give_the_greedy_tokens(drafts):
+    """Drafted tokens that are not accepted leave the cache: the tokens and the number cached are those of greedy decoding."""
+    model = _llama()
+    g = torch.Generator().manual_seed(2)
+    part = torch.randint(0, 128, (1, 4), generator=g)
+    prompt = torch.cat([part, torch.randint(0, 128, (1, 5), generator=g), part], 1)
+    if drafts.pop("assistant", None):
+        torch.manual_seed(3)
+        drafts["assistant_model"] = transformers.LlamaForCausalLM(transformers.LlamaConfig(
+            hidden_size=32, intermediate_size=48, num_hidden_layers=1, num_attention_heads=2, vocab_size=128)).eval()
+    got, lengths = [], []
+    for kw in ({}, drafts):
+        cache = kv4_cache(model, 1, 64, 32)
+        got.append(model.generate(prompt, attention_mask=torch.ones_like(prompt), past_key_values=cache, max_new_tokens=12,
+                                  do_sample=False, eos_token_id=None, pad_token_id=0, **kw))
+        lengths.append(cache.get_seq_length())
+    assert torch.equal(got[0], got[1])
+    assert lengths == [24, 24]
