@@ -18,7 +18,7 @@ from transformers.masking_utils import AttentionMaskInterface, causal_mask_funct
 from .attention import KV4Cache, kv4_append, kv4_attention, prompt_attention
 
 NAME = "crispybits"
-_LAYER = "_crispybits_kv4_layer"          # where a layer's update leaves itself on the keys it returns
+_LAYER = "_crispybits_kv4_layer"          # where a layer's update leaves itself on the keys and values it returns
 
 
 class KV4Layer(CacheLayerMixin):
@@ -41,8 +41,12 @@ class KV4Layer(CacheLayerMixin):
         k, v = (t.transpose(1, 2).reshape(b * s, heads, d) for t in (key_states, value_states))
         kv4_append(self.cache, k, v, o.block_table[:b], o.lengths(n)[:b], None if s == 1 else o.starts(b, s))
         self.seen = n
-        setattr(key_states, _LAYER, self)
-        return key_states, value_states
+        # Behind earlier tokens the keys and values only stand for the cached ones (a view of the new ones, as long as all of
+        # them): what a model makes of them is no longer this layer's, and too long to be taken for the new tokens' own.
+        out = (key_states, value_states) if n == s else tuple(t[:, :, :1].expand(-1, -1, n, -1) for t in (key_states, value_states))
+        for t in out:
+            setattr(t, _LAYER, self)
+        return out
 
     def get_mask_sizes(self, query_length: int):
         return self.seen + query_length, 0
@@ -137,11 +141,12 @@ def _attend(module, query, key, value, attention_mask, scaling=None, dropout=0.0
     b, heads, s, d = query.shape
     q = query.transpose(1, 2)
     layer = getattr(key, _LAYER, None)
-    if layer is not None and layer.seen > s:
+    if layer is not None and layer.seen > s and getattr(value, _LAYER, None) is layer:
         o = layer.owner
         return kv4_attention(q, layer.cache, o.block_table[:b], o.lengths(layer.seen)[:b], scale=scaling), None
     if key.shape[2] != s:
-        raise ValueError("crispybits attention over earlier tokens needs a PagedKV4Cache as past_key_values")
+        raise ValueError("crispybits attention over earlier tokens needs a PagedKV4Cache as past_key_values, and the keys and "
+                         "values that its update returned unchanged")
     k, v = (t.transpose(1, 2).reshape(b * s, -1, d) for t in (key, value))
     cu = layer.owner.starts(b, s) if layer is not None else _starts(b, s, q.device)
     return prompt_attention(q.reshape(b * s, heads, d), k, v, cu, s, scale=scaling).view(b, s, heads, d), None

@@ -1,5 +1,5 @@
-"""``PagedKV4Cache`` under the rules that Hugging Face's caches follow, on the CPU oracle in float64: what a crop keeps, and
-generation with drafted tokens that are checked and dropped."""
+"""``PagedKV4Cache`` under the rules that Hugging Face's caches follow, on the CPU oracle in float64: what a crop keeps,
+generation with drafted tokens that are checked and dropped, and models that do more to keys or scores than the ops know."""
 from types import SimpleNamespace
 
 import pytest
@@ -72,3 +72,40 @@ def test_checked_drafts_give_the_greedy_tokens(drafts):
         lengths.append(cache.get_seq_length())
     assert torch.equal(got[0], got[1])
     assert lengths == [24, 24]
+
+
+def test_keys_changed_behind_the_update_are_refused():
+    """JetMoe repeats keys and values after the cache took them: a prompt attends to them as they are, a later token, for
+    which they stand for the cached ones, is refused rather than attending to itself alone."""
+    torch.manual_seed(0)
+    cfg = transformers.JetMoeConfig(hidden_size=64, intermediate_size=64, num_hidden_layers=2, num_key_value_heads=2, kv_channels=16,
+                                    num_local_experts=4, num_experts_per_tok=2, vocab_size=128)
+    plain = transformers.JetMoeForCausalLM(cfg).eval()
+    tokens = torch.randint(0, 128, (1, 9), generator=torch.Generator().manual_seed(4))
+    with torch.no_grad():
+        want = plain(tokens).logits
+        model = install_attention(plain)
+        cache = kv4_cache(model, 1, 32, 32)
+        torch.testing.assert_close(model(tokens, past_key_values=cache).logits, want, atol=1e-4, rtol=1e-4)
+        with pytest.raises(ValueError, match="needs a PagedKV4Cache.*unchanged"):
+            model(tokens[:, :1], past_key_values=cache)
+
+
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_a_copy_of_what_the_update_returned_is_refused(what):
+    from crispybits_kernels import hf_attention as H
+    model = _llama()
+    cache = kv4_cache(model, 1, 32, 32)
+    g = torch.Generator().manual_seed(5)
+    new = lambda n: [torch.randn(1, 2, n, 16, generator=g).double() for _ in range(2)]     # noqa: E731
+    module = SimpleNamespace(is_causal=True)
+    q = torch.randn(1, 4, 5, 16, generator=g).double()
+    k, v = cache.update(*new(5), 0)
+    first = H._attend(module, q, k, v, None)[0]
+    assert torch.equal(H._attend(module, q, k.clone(), v.clone(), None)[0], first)           # a prompt holds all it needs
+    k, v = cache.update(*new(1), 0)
+    assert k.shape == v.shape == (1, 2, 6, 16)                                               # as a cache's keys and values are
+    assert H._attend(module, q[:, :, :1], k, v, None)[0].shape == (1, 1, 4, 16)
+    k, v = (t.clone() if what == n else t for n, t in (("key", k), ("value", v)))
+    with pytest.raises(ValueError, match="needs a PagedKV4Cache.*unchanged"):
+        H._attend(module, q[:, :, :1], k, v, None)
