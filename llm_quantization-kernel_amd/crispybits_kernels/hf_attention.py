@@ -5,8 +5,8 @@
 and values as they come and stores them in 4 bits; every later token attends to what is stored, its own included.
 Without a ``PagedKV4Cache`` every call must hold whole sequences (``use_cache=False``).
 
-The attention is causal and unpadded: a batch with padding, a mask of its own, a sliding window or dropout raises
-ValueError.  Sequences of one batch have one length.  Needs transformers (imported here, not by the package).
+The attention is causal and unpadded: a batch with padding, a mask of its own, a sliding window, dropout, capped scores,
+sinks or position biases raises ValueError.  Sequences of one batch have one length.  Needs transformers (imported here, not by the package).
 """
 from __future__ import annotations
 
@@ -19,6 +19,8 @@ from .attention import KV4Cache, kv4_append, kv4_attention, prompt_attention
 
 NAME = "crispybits"
 _LAYER = "_crispybits_kv4_layer"          # where a layer's update leaves itself on the keys and values it returns
+# arguments by which models ask for more than causal softmax attention
+_OTHER = ("softcap", "s_aux", "position_bias", "head_mask", "indices", "block_indices", "cu_seq_lens_q", "cu_seq_lens_k")
 
 
 class KV4Layer(CacheLayerMixin):
@@ -139,6 +141,9 @@ def _attend(module, query, key, value, attention_mask, scaling=None, dropout=0.0
     if kwargs.get("sliding_window") is not None:
         raise ValueError("crispybits attention has no sliding window")
     b, heads, s, d = query.shape
+    other = [n for n in _OTHER if kwargs.get(n) is not None]
+    if other or (s > 1 and kwargs.get("is_causal") is False):
+        raise ValueError(f"crispybits attention is plainly causal softmax attention: no {', '.join(other) or 'is_causal=False'}")
     q = query.transpose(1, 2)
     layer = getattr(key, _LAYER, None)
     if layer is not None and layer.seen > s and getattr(value, _LAYER, None) is layer:

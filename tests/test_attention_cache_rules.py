@@ -109,3 +109,16 @@ def test_a_copy_of_what_the_update_returned_is_refused(what):
     k, v = (t.clone() if what == n else t for n, t in (("key", k), ("value", v)))
     with pytest.raises(ValueError, match="needs a PagedKV4Cache.*unchanged"):
         H._attend(module, q[:, :, :1], k, v, None)
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=30.0), dict(s_aux=torch.zeros(4)), dict(sliding_window=8), dict(is_causal=False),
+                                dict(position_bias=torch.zeros(1, 4, 5, 5)), dict(indices=torch.zeros(1, 5, 2)),
+                                dict(cu_seq_lens_q=torch.tensor([0, 2, 5]))])
+def test_other_attentions_are_refused(kw):
+    """Arguments that would change the result are not dropped."""
+    from crispybits_kernels import hf_attention as H
+    q = torch.zeros(1, 4, 5, 16)
+    module = SimpleNamespace(is_causal=True)
+    with pytest.raises(ValueError, match="crispybits attention"):
+        H._attend(module, q, q, q, None, **kw)
+    H._attend(module, q, q, q, None, **{k: None for k in kw}, position_ids=torch.arange(5)[None], use_cache=True)
