@@ -28,7 +28,7 @@ class KV4Layer(CacheLayerMixin):
 
     def __init__(self, owner: "PagedKV4Cache", cache: KV4Cache):
         super().__init__()
-        self.owner, self.cache, self.seen = owner, cache, 0
+        self.owner, self.cache, self.seen, self.batch = owner, cache, 0, 0      # tokens and sequences held
         self.is_initialized = True
 
     def lazy_initialization(self, key_states, value_states):
@@ -40,9 +40,11 @@ class KV4Layer(CacheLayerMixin):
         n = self.seen + s
         if b > o.sequences or n > o.tokens:
             raise ValueError(f"{b} sequences of {n} tokens do not fit a cache of {o.sequences} x {o.tokens}")
+        if self.seen and b != self.batch:
+            raise ValueError(f"the cache holds {self.batch} sequences, not {b}")
         k, v = (t.transpose(1, 2).reshape(b * s, heads, d) for t in (key_states, value_states))
         kv4_append(self.cache, k, v, o.block_table[:b], o.lengths(n)[:b], None if s == 1 else o.starts(b, s))
-        self.seen = n
+        self.seen, self.batch = n, b
         # Behind earlier tokens the keys and values only stand for the cached ones (a view of the new ones, as long as all of
         # them): what a model makes of them is no longer this layer's, and too long to be taken for the new tokens' own.
         out = (key_states, value_states) if n == s else tuple(t[:, :, :1].expand(-1, -1, n, -1) for t in (key_states, value_states))
@@ -74,6 +76,7 @@ class KV4Layer(CacheLayerMixin):
             raise ValueError("more sequences than the cache has room for")
         p = self.cache.pages.view(self.owner.sequences, -1, *self.cache.pages.shape[1:])
         p[:n] = p.index_select(0, indices.to(p.device))
+        self.batch = n
 
     reorder_cache = batch_select_indices
 

@@ -122,3 +122,24 @@ def test_other_attentions_are_refused(kw):
     with pytest.raises(ValueError, match="crispybits attention"):
         H._attend(module, q, q, q, None, **kw)
     H._attend(module, q, q, q, None, **{k: None for k in kw}, position_ids=torch.arange(5)[None], use_cache=True)
+
+
+def test_a_batch_keeps_its_size():
+    """A later token of more or fewer sequences than the cached ones is refused; choosing sequences changes their number."""
+    model = _llama()
+    tokens = torch.randint(0, 128, (3, 5), generator=torch.Generator().manual_seed(6))
+    with torch.no_grad():
+        cache = kv4_cache(model, 3, 32, 32)
+        model(tokens[:2], past_key_values=cache)
+        for b in (1, 3):
+            with pytest.raises(ValueError, match="holds 2 sequences"):
+                model(tokens[:b, :1], past_key_values=cache)
+        assert cache.get_seq_length() == 5
+        cache.batch_select_indices(torch.tensor([1]))
+        got = model(tokens[1:2, :1], past_key_values=cache).logits
+        one = kv4_cache(model, 1, 32, 32)
+        model(tokens[1:2], past_key_values=one)
+        torch.testing.assert_close(got, model(tokens[1:2, :1], past_key_values=one).logits, atol=1e-5, rtol=1e-5)
+        cache.reset()
+        model(tokens, past_key_values=cache)
+        assert cache.get_seq_length() == 5
