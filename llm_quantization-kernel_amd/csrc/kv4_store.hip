@@ -100,10 +100,12 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], int lane, int
     hi = row_best<W, true>(hi);
     const uint64_t odd = __builtin_amdgcn_ballot_w64(!fine);
     const double r = (double)hi - (double)lo;
-    // z = rint(-15 lo / r), near 0 .. 15; r / 15 by its reciprocal and one correction, which rounds as the division
-    const float zt = -15.f * ((float)((double)lo * 0x1p-64) / (float)(r * 0x1p-64));
+    // z = rint(-15 lo / r), near 0 .. 15, in fp32 of the halves (no overflow): off by three roundings, 15 x 3 x 2^-24 < 3e-6,
+    // where r is not so small that halves lose bits; r / 15 by its reciprocal and one correction, which rounds as the division
+    const float rh = 0.5f * hi - 0.5f * lo;
+    const float zt = -15.f * (0.5f * lo / rh);
     float zr = r > 0.0 ? __builtin_rintf(zt) : 0.f;
-    if (__builtin_amdgcn_ballot_w64(r > 0.0 && !(__builtin_fabsf(zt - zr) < NEAR_HALF)) != 0)
+    if (__builtin_amdgcn_ballot_w64(r > 0.0 && !(__builtin_fabsf(zt - zr) < NEAR_HALF && rh >= 0x1p-100f)) != 0)
         zr = r > 0.0 ? (float)__builtin_rint(-15.0 * (double)lo / r) : 0.f;
     const double fifteenth = 1.0 / 15.0, q0 = r * fifteenth;
     const double fifth = __builtin_fma(__builtin_fma(-15.0, q0, r), fifteenth, q0);
