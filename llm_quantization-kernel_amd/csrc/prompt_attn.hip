@@ -7,8 +7,9 @@
 // way.  v_mfma_f32_32x32x16 gives a lane one row's column of S^T (tokens 8 i + 4 (lane / 32) + 0..3), which is the
 // operand layout of w for the tokens in that order, so w stays in its lane; V^T is read transposed from LDS
 // (ds_read_b64_tr_b16) in the same token order.  The running reference M of a row moves only when a tile's
-// largest score exceeds it by 8 (w <= 2^8 then, in range of fp16; sums are fp32), and stays a whole number, so that what it
-// scales is exact.  w is rounded to the type (nearest even): the products' operand.
+// largest score exceeds it by 8 (w <= 2^8 then, 2^15 in fp16, in range; sums are fp32), and stays a whole number, so that what it
+// scales is exact.  w is rounded to the type (nearest even): the products' operand.  l sums it unrounded: the
+// roundings, of either sign, average out, and taking each w back from its pair would cost two more instructions a pair.
 //
 // Bound: a tile of a wave costs 32 matrix instructions of 32 cycles (D = 128) and about as many cycles of vector
 // instructions (the softmax's, the same for any D); two waves a SIMD overlap them in part.  8192 rows, 32/8 heads, bf16:
@@ -34,6 +35,10 @@ constexpr int ROWS = 32 * WAVES;       // query rows of a workgroup
 constexpr int KT = 64;                 // tokens of a tile
 constexpr float LOW = -1e30f;
 constexpr float SLACK = 8.f;
+// Weights stand 2^UP above their reference: fp16 uses its range up to 2^15, so that what is denormal, or lost, lies 2^-20, or
+// 2^-31, below the largest weight rather than 2^-13 and 2^-24 (thirty thousand tokens of 2^-25 each count)
+template <int DT>
+constexpr float UP = DT == DT_F16 ? 7.f : 0.f;
 
 template <int DT>
 __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
@@ -270,10 +275,11 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
             }
         };
         auto weights = [&](const f16v& s, int i) {
+            const float at = UP<DT> - M;
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cc, -M));
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], cc, -M));
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cc, at));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], cc, at));
                 l += x + y;
                 w[2 * i + (j >> 3)][(j & 7) >> 1] = pack2<DT>(x, y);
             }
