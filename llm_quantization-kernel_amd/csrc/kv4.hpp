@@ -114,6 +114,16 @@ struct Kv4AttnArgs {
 };
 hipError_t launch_kv4_attn(const Kv4AttnArgs& A, int dt, hipStream_t stream);
 
+// From here on a running reference is too far from zero for s c - M as one FMA: the product's rest, up to half a last place
+// of M, would go into the exponent.
+constexpr float FAR = 0x1p24f;
+// s c, rounded, minus M
+__device__ __forceinline__ float less_rounded(float s, float c, float M) {
+#pragma clang fp contract(off)
+    const float p = s * c;
+    return p - M;
+}
+
 // prompt_attn.hip, prompt_attn_f32.hip
 struct PromptArgs {
     const void *q, *k, *v;

@@ -33,7 +33,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int WAVES = 4;
 constexpr int ROWS = 32 * WAVES;       // query rows of a workgroup
 constexpr int KT = 64;                 // tokens of a tile
-constexpr float LOW = -1e30f;
+constexpr float LOW = -0x1.fffffep127f;        // reference of a row that has seen nothing
 constexpr float SLACK = 8.f;
 // Weights stand 2^UP above their reference: fp16 uses its range up to 2^15, so that what is denormal, or lost, lies 2^-20, or
 // 2^-31, below the largest weight rather than 2^-13 and 2^-24 (thirty thousand tokens of 2^-25 each count)
@@ -188,6 +188,10 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
     for (int i = 0; i < DT32; ++i) acc[i] = zero16();
     float M = LOW, l = 0.f;
     const float cc = A.scale * 1.44269504088896341f;
+    // Exponents are s ca + at, in one FMA.  Where M is FAR from zero its product is not a float to within the exponents' range:
+    // there the rounded product minus M takes s's place.
+    float ca = cc, at = 0.f;
+    bool far = false;                                             // some row of the wave is so
 
     // LDS addresses of this lane's operands: K row n (32 rows on: the same places) at step s; V^T of d tile i, two
     // transposed reads of four tokens a token step.  An exclusive or takes a turned row from step to step.
@@ -258,7 +262,7 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
             const uint32_t u = __float_as_uint(top);
             const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
             top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * cc;
-            if (__builtin_amdgcn_ballot_w64(top > M + SLACK) != 0) {
+            if (far || __builtin_amdgcn_ballot_w64(top > M + SLACK) != 0) {
                 const float to = top > M + SLACK ? __builtin_ceilf(top) : M;       // whole: what it scales stays exact
                 const float f = __builtin_amdgcn_exp2f(M - to);
                 M = to;
@@ -272,14 +276,21 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         w[k][e] = pack2<DT>(half_of<DT>(w[k][e]) * f, half_of<DT>(w[k][e] >> 16) * f);
+                const bool apart = !(__builtin_fabsf(M) < FAR);
+                ca = apart ? 1.f : cc;
+                at = apart ? UP<DT> : UP<DT> - M;
+                far = __builtin_amdgcn_ballot_w64(apart) != 0;
+                if (far) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[j] = apart ? less_rounded(s[j], cc, M) : s[j];
+                }
             }
         };
         auto weights = [&](const f16v& s, int i) {
-            const float at = UP<DT> - M;
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cc, at));
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], cc, at));
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], ca, at));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], ca, at));
                 l += x + y;
                 w[2 * i + (j >> 3)][(j & 7) >> 1] = pack2<DT>(x, y);
             }

@@ -22,7 +22,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int WAVES = 4;
 constexpr int ROWS = 32 * WAVES;
 constexpr int KT = 32;
-constexpr float LOW = -1e30f;
+constexpr float LOW = -0x1.fffffep127f;        // reference of a row that has seen nothing
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -152,10 +152,17 @@ __global__ __launch_bounds__(64 * WAVES, 1) void prompt_attn_f32_kernel(PromptAr
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[i][j] *= f;
         }
+        float ca = cc, cb = cl, m = -M;
+        const bool apart = !(__builtin_fabsf(M) < FAR);
+        if (__builtin_amdgcn_ballot_w64(apart) != 0) {  // as in prompt_attn.hip: the rounded product minus M for s
+            ca = apart ? 1.f : cc, cb = apart ? 0.f : cl, m = apart ? 0.f : m;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = apart ? less_rounded(s[j], cc, M) : s[j];
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const float at = s[j] > -__builtin_inff() ? __builtin_fmaf(s[j], cl, -M) : -M;
-            s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cc, at));
+            const float at = s[j] > -__builtin_inff() ? __builtin_fmaf(s[j], cb, m) : m;
+            s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], ca, at));
             l += s[j];
         }
         // masked places take no part whatever they hold: on the diagonal, infinities and NaN go in as zeros and
