@@ -14,9 +14,10 @@
 // q is scaled by a power of two per row, to values below 2^11, so that its fp16 is exact for fp16 and
 // bf16 q (fp32 q and w go as two fp16 terms each); where the stored pairs count 16 times, q is held / 16, and
 // w takes the 1/16 in its exponent.  w must fit fp16 at any scale s': the running reference M of a row
-// bounds score + log2 s' over the tokens seen, w = 2^(score - M + 12) s', so that w < 2^16 and 26 bits
-// below the largest still count; the sum of p is held with the same factor.  M moves only when it would
-// have to by 3 or more (the accumulators are rescaled then).
+// bounds score + log2 s' of each token seen, w = 2^(score - M + 12) s', so that w < 2^15, the largest is 2^10 or
+// more, and only what lies 2^31 below it is lost; the sum of p is held with the same factor, of unrounded p (the
+// roundings of w, of either sign, average out).  M moves only when it would have to by 3 or more (the accumulators are
+// rescaled then).
 //
 // Work: a unit is a sequence, kv head and tile of 16 query rows, of as many blocks as the sequence has (one at
 // least, whose workgroup writes the zeros of an empty one).  The blocks of all units stand in one row, sequence by
@@ -43,7 +44,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
 constexpr float LOW = -1e30f;          // reference of a row that has seen nothing
-constexpr float HEADROOM = 12.f;       // w < 2^(HEADROOM + 3 + 1)
+constexpr float HEADROOM = 12.f;       // w < 2^(HEADROOM + SLACK)
 constexpr float SLACK = 3.f;
 
 union Op {
@@ -486,11 +487,11 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                     sv[j] = seen ? sv[j] : 0.f;
                 }
             }
-            float ym = y[0], sm = sv[0];
+            // what score + log2 s' stays below, token by token (the largest of each would pass every real weight by their spread)
+            float bound = -__builtin_inff();
 #pragma unroll
-            for (int j = 1; j < 8; ++j) ym = fmaxf(ym, y[j]), sm = fmaxf(sm, sv[j]);
-            // score + log2 s' is below this for every token of the lane
-            float bound = ym * cc + (float)max(__builtin_amdgcn_frexp_expf(sm), -90);
+            for (int j = 0; j < 8; ++j)
+                bound = fmaxf(bound, __builtin_fmaf(y[j], cc, (float)max(__builtin_amdgcn_frexp_expf(sv[j]), -90)));
             bound = group_max(bound);
             if (__builtin_amdgcn_ballot_w64(bound > M + SLACK) != 0) {
                 const float to = bound > M + SLACK ? __builtin_ceilf(bound) : M;     // whole: what it scales stays exact
