@@ -56,7 +56,7 @@ int cbk_kv4_read(const int32_t* pages, int64_t num_pages, int64_t kv_heads, int 
 
 /* out[b, i, h] = softmax(scale q[b, i, h] . K^T) V over sequence b's tokens 0 .. seq_lens[b] - t + i, for its t
  * newest tokens: q and out contiguous [num_seqs, t, heads, head_dim].  A query that sees no token gives
- * zeros.  scale > 0.  partial: cbk_kv4_attention_partial_floats(...) fp32 elements (0: none needed), scratch of
+ * zeros.  0 < scale <= 2^127.  partial: cbk_kv4_attention_partial_floats(...) fp32 elements (0: none needed), scratch of
  * this call alone. */
 int64_t cbk_kv4_attention_partial_floats(int64_t num_seqs, int64_t t, int64_t heads, int64_t kv_heads, int head_dim,
                                          int64_t page_size, int64_t table_width);
@@ -70,7 +70,7 @@ int cbk_kv4_attention(const void* q, int dtype, int64_t num_seqs, int64_t t, int
  * (0 < max_seqlen <= rows) bounds every sequence's length; rows of a longer one past it are not computed;
  * ceil(max_seqlen / 128) (num_seqs + 1) heads must be below 2^24.  Rows of no
  * sequence (behind the last) are set to zero when zero_tail, else left as they were.  Places that the mask
- * hides take no part whatever they hold.  scale > 0. */
+ * hides take no part whatever they hold.  0 < scale <= 2^127. */
 int cbk_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t rows, int64_t heads,
                          int64_t kv_heads, int head_dim, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                          int64_t v_row, int64_t v_head, const int32_t* cu_seqlens, int64_t num_seqs,

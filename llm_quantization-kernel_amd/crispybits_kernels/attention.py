@@ -89,7 +89,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, s
 
     q is [sequences, heads, head_dim] (one new token each) or [sequences, t, heads, head_dim] (the t newest,
     which the cache already holds): query i sees positions up to ``seq_lens - t + i``.  Query heads are
-    grouped over the cache's kv heads.  ``scale`` (positive) defaults to head_dim ** -0.5.  A query that sees nothing
+    grouped over the cache's kv heads.  ``scale`` (positive, at most 2^127) defaults to head_dim ** -0.5.  A query that sees nothing
     (an idle slot) gives zeros.  Tokens whose table entry names no page take no part."""
     if q.dim() not in (3, 4):
         raise ValueError("q must be [sequences, heads, head_dim] or [sequences, new tokens, heads, head_dim]")
@@ -110,7 +110,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     head_dim] (fp16 / bf16 / fp32, rows and heads strided as they come), row i of a sequence attending to its rows
     0 .. i.  ``cu_seqlens`` int32 [sequences + 1] holds the sequences' first rows and the end of the last.
     ``max_seqlen`` is at least the longest sequence's length (default: all rows; a tight bound launches less).
-    ``scale`` (positive) defaults to head_dim ** -0.5.  Rows behind the last sequence come back as zeros, or stay as
+    ``scale`` (positive, at most 2^127) defaults to head_dim ** -0.5.  Rows behind the last sequence come back as zeros, or stay as
     they were in ``out``.  What the causal mask hides takes no part, infinities and NaN included."""
     if q.dim() != 3:
         raise ValueError("q must be [rows, heads, head_dim]")

@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "cbk_host.hpp"
 #include "cbk_kernels.hpp"
@@ -40,6 +39,12 @@ int check_strides(const char* what, int dtype, int64_t row, int64_t head) {
     if (row < 0 || head < 0 || row % unit != 0 || head % unit != 0)
         return fail(CBK_EINVAL, "%s: rows of a head must be 16-byte aligned", what);
     if (row > MAX_ROW_STRIDE) return fail(CBK_EINVAL, "%s: row strides are at most 2^23 elements", what);
+    return CBK_OK;
+}
+
+// scale log2 e is an fp32 factor of the kernels
+int check_scale(const char* what, float scale) {
+    if (!(scale > 0.f && scale <= 0x1p127f)) return fail(CBK_EINVAL, "%s: scale must be positive and at most 2^127", what);
     return CBK_OK;
 }
 
@@ -182,7 +187,7 @@ int cbk_kv4_attention(const void* q, int dtype, int64_t num_seqs, int64_t t, int
     if (int e = view(what, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_width, seq_lens, num_seqs,
                      A.c))
         return e;
-    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(CBK_EINVAL, "%s: scale must be positive and finite", what);
+    if (int e = check_scale(what, scale)) return e;
     if (t < 0 || t > MOST || t * heads > MOST) return fail(CBK_EINVAL, "%s: bad number of new tokens", what);
     if (num_seqs == 0 || t == 0) return CBK_OK;
     if (!q || !out) return fail(CBK_EINVAL, "%s: q and out must be non-null", what);
@@ -218,7 +223,7 @@ int cbk_prompt_attention(const void* q, const void* k, const void* v, int dtype,
     if (int e = check_strides(what, dtype, v_row, v_head)) return e;
     if (rows < 0 || rows > MOST) return fail(CBK_EINVAL, "%s: bad number of rows", what);
     if (num_seqs < 0 || num_seqs > MOST_GRID) return fail(CBK_EINVAL, "%s: at most %d sequences", what, (int)MOST_GRID);
-    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(CBK_EINVAL, "%s: scale must be positive and finite", what);
+    if (int e = check_scale(what, scale)) return e;
     if (rows == 0) return CBK_OK;
     if (num_seqs == 0) return fail(CBK_EINVAL, "%s: rows without a sequence", what);
     if (max_seqlen <= 0 || max_seqlen > rows)

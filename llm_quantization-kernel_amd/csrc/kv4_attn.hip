@@ -43,7 +43,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
-constexpr float LOW = -1e30f;          // reference of a row that has seen nothing
+constexpr float LOW = -0x1.fffffep127f;        // reference of a row that has seen nothing
 constexpr float HEADROOM = 12.f;       // w < 2^(HEADROOM + SLACK)
 constexpr float SLACK = 3.f;
 
@@ -251,7 +251,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float* p, long
 template <int DT>
 __device__ __forceinline__ void combine(const Kv4AttnArgs& A, CombineLds& L, const Parts& P, int b, int h, int tile) {
     constexpr int EARLY = 8;
-    const int D = A.c.d, cols = min(A.cols, A.rows - 16 * tile), tid = threadIdx.x;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));                                // its places are found here, not held in registers all along
+    const int D = A.c.d, cols = min(A.cols, A.rows - 16 * tile);
     const int col = tid & 15, s0 = tid >> 4;
     const __amdgpu_buffer_rsrc_t sums = buffer_of(part_sums(A, 2 * P.first), 2l * P.count * A.cols * D);
     const __amdgpu_buffer_rsrc_t rows = buffer_of(part_rows(A, 2 * P.first), 4l * P.count * A.cols);
@@ -398,7 +400,9 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
 
         // q scaled to below 2^11, and its sum
         Op q[TERMS][NS];
-        float cc, cl = 0.f, qsum = 0.f;
+        float cc, cl = 0.f, qsum = 0.f;                // exponents are y cc (+ y cl) + at
+        const double c2 = (double)A.scale * 1.44269504088896340736;
+        const float cm = __builtin_amdgcn_frexp_mantf((float)c2);
         {
             float x[NS][8];
             float top = 0.f;
@@ -435,8 +439,9 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                 }
             if constexpr (!EXACT) qsum = group_sum(qsum) * 0x1p-22f;
             // scale log2 e; for fp32 in two terms: its rounding would bend every score by 2^-24 of itself
-            const double c2 = (double)A.scale * 1.44269504088896340736;
-            cc = __builtin_ldexpf((float)c2, UP - 11 + e);
+            const int ce = UP - 11 + e + __builtin_amdgcn_frexp_expf((float)c2);
+            cc = __builtin_ldexpf(cm, ce);
+            red_l[wave][n] = (float)ce;                // cc is cm 2^ce, kept there until the waves meet
             if constexpr (EXACT) cl = __builtin_ldexpf((float)(c2 - (double)(float)c2), UP - 11 + e);
         }
 
@@ -444,6 +449,11 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
 #pragma unroll
         for (int i = 0; i < TILES; ++i) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
         float M = LOW, la = 0.f, lb = 0.f;
+        // A row with a reference FAR from zero stands apart: its exponents are the rounded score minus M, the largest score
+        // alone, and minus E, the largest exponent of a value scale among scores near it (sums of such scores and
+        // exponents would not be floats).  far: some row of the wave does.
+        float at = HEADROOM;                           // HEADROOM - M; of a row apart HEADROOM - E
+        bool apart = !(cc < 0x1p126f), far = __builtin_amdgcn_ballot_w64(apart) != 0;
 
         while (blk < last) {
             bool next_there;
@@ -493,10 +503,32 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
             for (int j = 0; j < 8; ++j)
                 bound = fmaxf(bound, __builtin_fmaf(y[j], cc, (float)max(__builtin_amdgcn_frexp_expf(sv[j]), -90)));
             bound = group_max(bound);
-            if (__builtin_amdgcn_ballot_w64(bound > M + SLACK) != 0) {
-                const float to = bound > M + SLACK ? __builtin_ceilf(bound) : M;     // whole: what it scales stays exact
-                const float f = __builtin_amdgcn_exp2f(M - to);
+            if (far || __builtin_amdgcn_ballot_w64(bound > M + SLACK) != 0) {
+                const bool moves = !apart && bound > M + SLACK, joins = moves && !(__builtin_fabsf(bound) < FAR);
+                const float E = apart ? HEADROOM - at : 0.f;
+                float to = moves ? __builtin_ceilf(bound) : M, Eto = 0.f;            // whole: what they scale stays exact
+                far = __builtin_amdgcn_ballot_w64(apart || joins) != 0;
+                if (__builtin_expect(far, 0)) {
+                    const int ce = (int)red_l[wave][n];
+                    float top = M;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, __builtin_ldexpf(y[j] * cm, ce));
+                    top = group_max(top);
+                    int ex = -90;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        ex = max(ex, __builtin_ldexpf(y[j] * cm, ce) >= top - 256.f ? (int)(__float_as_uint(sv[j]) >> 23) - 126 : -90);
+                    Eto = fmaxf(group_max((float)ex), apart && M >= top - 256.f ? E : -90.f);
+                    apart |= joins;
+                    to = apart ? top : to;
+                    Eto = apart ? Eto : 0.f;
+                    cc = apart ? 1.f : cc, cl = apart ? 0.f : cl;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = apart ? __builtin_ldexpf(y[j] * cm, ce) - top : y[j];
+                }
+                const float f = __builtin_amdgcn_exp2f(M - to + (E - Eto));
                 M = to;
+                at = HEADROOM - (apart ? Eto : to);
                 la *= f, lb *= f;
 #pragma unroll
                 for (int i = 0; i < TILES; ++i)
@@ -505,13 +537,13 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
 #pragma unroll
                 for (int j = 0; j < 4; ++j) accz[j] *= f;
             }
-            const float ma = HEADROOM - M, mb = EXACT ? ma : HEADROOM - 4.f - M;
+            const float ma = at, mb = EXACT ? ma : ma - 4.f;
             float w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float at = (j & 2) ? mb : ma;
-                if constexpr (EXACT) at = y[j] > -__builtin_inff() ? __builtin_fmaf(y[j], cl, at) : at;
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, at));
+                float m = (j & 2) ? mb : ma;
+                if constexpr (EXACT) m = y[j] > -__builtin_inff() ? __builtin_fmaf(y[j], cl, m) : m;
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, m));
                 if (j & 2) lb += p;
                 else la += p;
                 w[j] = p * sv[j];
@@ -556,6 +588,17 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
 
         // the waves' rows meet
         float l = group_sum(EXACT ? la + lb : __builtin_fmaf(16.f, lb, la));
+        if (__builtin_expect(far, 0)) {                    // rows apart: sums at the reference M + HEADROOM alone
+            const int e = apart ? -(int)at : 0;
+            M += apart ? HEADROOM : 0.f;
+            l = __builtin_ldexpf(l, e);
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_ldexpf(acc[i][j], e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) accz[j] = __builtin_ldexpf(accz[j], e);
+        }
         if (g == 0) red_m[wave][n] = M, red_l[wave][n] = l;
         __syncthreads();
         float top = red_m[0][n];
