@@ -97,8 +97,10 @@ hipError_t launch_kv4_append(const Kv4StoreArgs& A, int dt, hipStream_t stream);
 hipError_t launch_kv4_read(const Kv4StoreArgs& A, int dt, hipStream_t stream);
 
 // kv4_attn.hip
-// Workgroups of the attention kernel that a CU holds: by its registers (up to 128 values three, fp32 at 128 and more two).
-__host__ __device__ constexpr int kv4_waves(int ns, int dt) { return ns < 4 || (ns == 4 && dt != DT_F32) ? 3 : 2; }
+// Workgroups of the attention kernel that a CU holds, by its registers.
+__host__ __device__ constexpr int kv4_waves(int ns, int dt) {
+    return dt == DT_F32 ? (ns <= 2 ? 3 : ns <= 4 ? 2 : 1) : ns <= 4 ? 3 : 2;
+}
 struct Kv4AttnArgs {
     Kv4View c;
     const void* q;             // [seqs, t, hq, d] contiguous, 16-byte aligned
@@ -116,7 +118,7 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs& A, int dt, hipStream_t stream);
 
 // From here on a running reference is too far from zero for s c - M as one FMA: the product's rest, up to half a last place
 // of M, would go into the exponent.
-constexpr float FAR = 0x1p24f;
+constexpr float FAR = 0x1p20f;
 // s c, rounded, minus M
 __device__ __forceinline__ float less_rounded(float s, float c, float M) {
 #pragma clang fp contract(off)

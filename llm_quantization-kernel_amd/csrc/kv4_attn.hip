@@ -12,12 +12,16 @@
 // more product, with the zero points as codes.
 //
 // q is scaled by a power of two per row, to values below 2^11, so that its fp16 is exact for fp16 and
-// bf16 q (fp32 q and w go as two fp16 terms each); where the stored pairs count 16 times, q is held / 16, and
+// bf16 q; where the stored pairs count 16 times, q is held / 16, and
 // w takes the 1/16 in its exponent.  w must fit fp16 at any scale s': the running reference M of a row
 // bounds score + log2 s' of each token seen, w = 2^(score - M + 12) s', so that w < 2^15, the largest is 2^10 or
 // more, and only what lies 2^31 below it is lost; the sum of p is held with the same factor, of unrounded p (the
 // roundings of w, of either sign, average out).  M moves only when it would have to by 3 or more (the accumulators are
 // rescaled then).
+// fp32 q and w go as three fp16 terms, 33 bits: a whole number below 2^11 and two of the rest, with sums of their own, and
+// codes with the zero point taken off.  Sums of whole numbers are exact in the matrix product, so the scores' own rounding
+// is what is left: 1e-7 of an output at 500 tokens, fp32 products of torch 5e-7.  (Two terms in one sum: up to 1e-5, at 14.6 us
+// instead of 16.1 for 5 sequences of 200..1501 tokens, 32 heads of 80; fp32 matrix instructions have a sixteenth of the rate.)
 //
 // Work: a unit is a sequence, kv head and tile of 16 query rows, of as many blocks as the sequence has (one at
 // least, whose workgroup writes the zeros of an empty one).  The blocks of all units stand in one row, sequence by
@@ -44,8 +48,10 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
 constexpr float LOW = -0x1.fffffep127f;        // reference of a row that has seen nothing
-constexpr float HEADROOM = 12.f;       // w < 2^(HEADROOM + SLACK)
 constexpr float SLACK = 3.f;
+// w < 2^(HEADROOM + SLACK): 2^15, in fp16's range; fp32's w below 2^11, whose whole part is one fp16 term
+template <int DT>
+constexpr float HEADROOM = DT == DT_F32 ? 8.f : 12.f;
 
 union Op {
     h8 v;
@@ -76,6 +82,13 @@ __device__ __forceinline__ h8 decode_exact(uint32_t w, h2 lo0, h2 hi0, h2 lo1, h
     o.u[2] = __builtin_bit_cast(uint32_t, pair_of((s & 0x003C003Cu) | 0x5C005C00u) + lo1);
     o.u[3] = __builtin_bit_cast(uint32_t, pair_of((s & 0x03C003C0u) | 0x4C004C00u) + hi1);
     return o.v;
+}
+
+// x of magnitude below 2^11 as a + b 2^-11 + c 2^-11, a and b whole numbers: products with codes sum up exactly in a
+// matrix product (24 bits below its largest term are kept), those of c to 2^-33 of the largest x.
+__device__ __forceinline__ void in_three(float x, _Float16& a, _Float16& b, _Float16& c) {
+    const float i = __builtin_rintf(x), r = (x - i) * 2048.f, k = __builtin_rintf(r);
+    a = (_Float16)i, b = (_Float16)k, c = (_Float16)(r - k);
 }
 
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -342,7 +355,8 @@ template <int NS, int DT>
 __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv4_attn_kernel(Kv4AttnArgs A) {
     constexpr int TILES = 2 * NS, DP = 32 * NS;
     constexpr bool EXACT = DT == DT_F32;
-    constexpr int TERMS = EXACT ? 2 : 1;
+    constexpr int TERMS = EXACT ? 3 : 1, SUMS = EXACT ? 2 : 1;
+    constexpr float HEAD = HEADROOM<DT>;
     constexpr int UP = EXACT ? 0 : 22;                 // codes in the products are c 2^-UP
     union Lds {
         float red[2][16][DP + 4];
@@ -426,16 +440,13 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float v = __builtin_ldexpf(x[s][j], 11 - e);
-                    const float u = !EXACT && (j & 2) ? v * 0.0625f : v;
-                    const _Float16 hi = (_Float16)u;
-                    q[0][s].h[j] = hi;
-                    float held = (float)hi;
-                    if constexpr (TERMS == 2) {
-                        const _Float16 lo = (_Float16)(u - held);
-                        q[1][s].h[j] = lo;
-                        held += (float)lo;
+                    if constexpr (EXACT) {
+                        in_three(v, q[0][s].h[j], q[1][s].h[j], q[2][s].h[j]);
+                    } else {
+                        const _Float16 h = (_Float16)((j & 2) ? v * 0.0625f : v);
+                        q[0][s].h[j] = h;
+                        qsum += (j & 2) ? (float)h * 16.f : (float)h;
                     }
-                    if constexpr (!EXACT) qsum += (j & 2) ? held * 16.f : held;
                 }
             if constexpr (!EXACT) qsum = group_sum(qsum) * 0x1p-22f;
             // scale log2 e; for fp32 in two terms: its rounding would bend every score by 2^-24 of itself
@@ -445,14 +456,14 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
             if constexpr (EXACT) cl = __builtin_ldexpf((float)(c2 - (double)(float)c2), UP - 11 + e);
         }
 
-        f4 acc[TILES], accz = {0.f, 0.f, 0.f, 0.f};
+        f4 acc[TILES * SUMS], accz = {0.f, 0.f, 0.f, 0.f};           // EXACT: whole parts, then the rest 2^11 times
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < TILES * SUMS; ++i) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
         float M = LOW, la = 0.f, lb = 0.f;
         // A row with a reference FAR from zero stands apart: its exponents are the rounded score minus M, the largest score
         // alone, and minus E, the largest exponent of a value scale among scores near it (sums of such scores and
         // exponents would not be floats).  far: some row of the wave does.
-        float at = HEADROOM;                           // HEADROOM - M; of a row apart HEADROOM - E
+        float at = HEAD;                               // HEAD - M; of a row apart HEAD - E
         bool apart = !(cc < 0x1p126f), far = __builtin_amdgcn_ballot_w64(apart) != 0;
 
         while (blk < last) {
@@ -462,7 +473,7 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
             float y[8], sv[8];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                f4 s = {0.f, 0.f, 0.f, 0.f};
+                f4 s = {0.f, 0.f, 0.f, 0.f}, rest = s;
 #pragma unroll
                 for (int st = 0; st < NS; ++st) {
                     if constexpr (EXACT) {
@@ -471,7 +482,8 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                         const h2 hi = h2{(_Float16)-16.f, (_Float16)-16.f} - h2{z, z};
                         const h8 kc = decode_exact(B.k[i][st], lo, hi, lo, hi);
                         s = mfma(kc, q[0][st].v, s);
-                        s = mfma(kc, q[1][st].v, s);
+                        rest = mfma(kc, q[1][st].v, rest);
+                        rest = mfma(kc, q[2][st].v, rest);
                     } else {
                         s = mfma(decode(B.k[i][st]), q[0][st].v, s);
                     }
@@ -479,7 +491,8 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t w = B.km[i][j];
-                    y[4 * i + j] = __uint_as_float(w) * (EXACT ? s[j] : __builtin_fmaf(-(float)(w & 15u), qsum, s[j]));
+                    y[4 * i + j] = __uint_as_float(w) * (EXACT ? __builtin_fmaf(rest[j], 0x1p-11f, s[j])
+                                                             : __builtin_fmaf(-(float)(w & 15u), qsum, s[j]));
                 }
             }
             // the next block's keys, under way from here on (kept behind the last use of this one's, in its registers)
@@ -505,7 +518,7 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
             bound = group_max(bound);
             if (far || __builtin_amdgcn_ballot_w64(bound > M + SLACK) != 0) {
                 const bool moves = !apart && bound > M + SLACK, joins = moves && !(__builtin_fabsf(bound) < FAR);
-                const float E = apart ? HEADROOM - at : 0.f;
+                const float E = apart ? HEAD - at : 0.f;
                 float to = moves ? __builtin_ceilf(bound) : M, Eto = 0.f;            // whole: what they scale stays exact
                 far = __builtin_amdgcn_ballot_w64(apart || joins) != 0;
                 if (__builtin_expect(far, 0)) {
@@ -528,31 +541,42 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                 }
                 const float f = __builtin_amdgcn_exp2f(M - to + (E - Eto));
                 M = to;
-                at = HEADROOM - (apart ? Eto : to);
+                at = HEAD - (apart ? Eto : to);
                 la *= f, lb *= f;
 #pragma unroll
-                for (int i = 0; i < TILES; ++i)
+                for (int i = 0; i < TILES * SUMS; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[i][j] *= f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) accz[j] *= f;
             }
-            const float ma = at, mb = EXACT ? ma : ma - 4.f;
             float w[8];
+            if constexpr (EXACT) {
+                // The whole part of the exponent apart: with it in one sum the fraction would keep 20 bits.
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float m = (j & 2) ? mb : ma;
-                if constexpr (EXACT) m = y[j] > -__builtin_inff() ? __builtin_fmaf(y[j], cl, m) : m;
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, m));
-                if (j & 2) lb += p;
-                else la += p;
-                w[j] = p * sv[j];
+                for (int j = 0; j < 8; ++j) {
+                    const float whole = __builtin_rintf(y[j] * cc);
+                    const float part = __builtin_fmaf(y[j], cl, __builtin_fmaf(y[j], cc, -whole));
+                    const float p = __builtin_ldexpf(__builtin_amdgcn_exp2f(part), (int)fmaxf(whole + at, -1000.f));
+                    w[j] = y[j] == -__builtin_inff() ? 0.f : p;
+                    la += w[j];
+                    w[j] *= sv[j];
+                }
+            } else {
+                const float ma = at, mb = ma - 4.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], cc, (j & 2) ? mb : ma));
+                    if (j & 2) lb += p;
+                    else la += p;
+                    w[j] = p * sv[j];
+                }
             }
             Op wo[TERMS], zo;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                wo[0].h[j] = (_Float16)w[j];
-                if constexpr (TERMS == 2) wo[1].h[j] = (_Float16)(w[j] - (float)wo[0].h[j]);
+                if constexpr (EXACT) in_three(w[j], wo[0].h[j], wo[1].h[j], wo[2].h[j]);
+                else wo[0].h[j] = (_Float16)w[j];
             }
             if constexpr (EXACT) {
                 h2 bias[4];                                // of tokens (0, 1), (2, 3), (4, 5), (6, 7)
@@ -567,7 +591,8 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                 for (int i = 0; i < TILES; ++i) {
                     const h8 vc = decode_exact(B.v[i], bias[0], bias[1], bias[2], bias[3]);
                     acc[i] = mfma(vc, wo[0].v, acc[i]);
-                    acc[i] = mfma(vc, wo[1].v, acc[i]);
+                    acc[TILES + i] = mfma(vc, wo[1].v, acc[TILES + i]);
+                    acc[TILES + i] = mfma(vc, wo[2].v, acc[TILES + i]);
                 }
             } else {
                 // zero points as codes: pairs (0,1), (4,5) plain, (2,3), (6,7) 16-fold
@@ -587,10 +612,16 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
         }
 
         // the waves' rows meet
-        float l = group_sum(EXACT ? la + lb : __builtin_fmaf(16.f, lb, la));
-        if (__builtin_expect(far, 0)) {                    // rows apart: sums at the reference M + HEADROOM alone
+        float l = group_sum(__builtin_fmaf(16.f, lb, la));
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_fmaf(acc[TILES + i][j], 0x1p-11f, acc[i][j]);
+        }
+        if (__builtin_expect(far, 0)) {                    // rows apart: sums at the reference M + HEAD alone
             const int e = apart ? -(int)at : 0;
-            M += apart ? HEADROOM : 0.f;
+            M += apart ? HEAD : 0.f;
             l = __builtin_ldexpf(l, e);
 #pragma unroll
             for (int i = 0; i < TILES; ++i)
