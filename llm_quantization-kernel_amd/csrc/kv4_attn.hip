@@ -15,9 +15,10 @@
 // bf16 q; where the stored pairs count 16 times, q is held / 16, and
 // w takes the 1/16 in its exponent.  w must fit fp16 at any scale s': the running reference M of a row
 // bounds score + log2 s' of each token seen, w = 2^(score - M + 12) s', so that w < 2^15, the largest is 2^10 or
-// more, and only what lies 2^31 below it is lost; the sum of p is held with the same factor, of unrounded p (the
-// roundings of w, of either sign, average out).  M moves only when it would have to by 3 or more (the accumulators are
-// rescaled then).
+// more, and only what lies 2^31 below it is lost; the sum of p is held with the same factor, of unrounded p.  For fp16
+// outputs w goes as two fp16 terms, 22 bits: one term's rounding is as large as the output's own (errors of 2.9e-4 against 2.1e-4,
+// at 37.2 against 39.5 us for the ragged batch of 32); for bf16 outputs it is an eighth of it.  M moves only when it
+// would have to by 3 or more (the accumulators are rescaled then).
 // fp32 q and w go as three fp16 terms, 33 bits: a whole number below 2^11 and two of the rest, with sums of their own, and
 // codes with the zero point taken off.  Sums of whole numbers are exact in the matrix product, so the scores' own rounding
 // is what is left: 1e-7 of an output at 500 tokens, fp32 products of torch 5e-7.  (Two terms in one sum: up to 1e-5, at 14.6 us
@@ -355,7 +356,7 @@ template <int NS, int DT>
 __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv4_attn_kernel(Kv4AttnArgs A) {
     constexpr int TILES = 2 * NS, DP = 32 * NS;
     constexpr bool EXACT = DT == DT_F32;
-    constexpr int TERMS = EXACT ? 3 : 1, SUMS = EXACT ? 2 : 1;
+    constexpr int TERMS = EXACT ? 3 : 1, SUMS = EXACT ? 2 : 1, W_TERMS = EXACT ? 3 : DT == DT_F16 ? 2 : 1;
     constexpr float HEAD = HEADROOM<DT>;
     constexpr int UP = EXACT ? 0 : 22;                 // codes in the products are c 2^-UP
     union Lds {
@@ -572,11 +573,12 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                     w[j] = p * sv[j];
                 }
             }
-            Op wo[TERMS], zo;
+            Op wo[W_TERMS], zo;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if constexpr (EXACT) in_three(w[j], wo[0].h[j], wo[1].h[j], wo[2].h[j]);
                 else wo[0].h[j] = (_Float16)w[j];
+                if constexpr (W_TERMS == 2) wo[1].h[j] = (_Float16)(w[j] - (float)wo[0].h[j]);
             }
             if constexpr (EXACT) {
                 h2 bias[4];                                // of tokens (0, 1), (2, 3), (4, 5), (6, 7)
@@ -602,8 +604,13 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
                     zo.u[2 * i + 1] = (__builtin_amdgcn_perm(B.vm[i][3], B.vm[i][2], 0x0C040C00u) & 0x000F000Fu) << 6;
                 }
                 accz = mfma(zo.v, wo[0].v, accz);
+                if constexpr (W_TERMS == 2) accz = mfma(zo.v, wo[1].v, accz);
 #pragma unroll
-                for (int i = 0; i < TILES; ++i) acc[i] = mfma(decode(B.v[i]), wo[0].v, acc[i]);
+                for (int i = 0; i < TILES; ++i) {
+                    const h8 vc = decode(B.v[i]);
+                    acc[i] = mfma(vc, wo[0].v, acc[i]);
+                    if constexpr (W_TERMS == 2) acc[i] = mfma(vc, wo[1].v, acc[i]);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
             B.load_v(next, lane);
