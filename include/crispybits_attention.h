@@ -70,7 +70,7 @@ int cbk_kv4_attention(const void* q, int dtype, int64_t num_seqs, int64_t t, int
  * (0 < max_seqlen <= rows) bounds every sequence's length; rows of a longer one past it are not computed;
  * ceil(max_seqlen / 128) (num_seqs + 1) heads must be below 2^24.  Rows of no
  * sequence (behind the last) are set to zero when zero_tail, else left as they were.  Places that the mask
- * hides take no part whatever they hold.  0 < scale <= 2^127. */
+ * hides take no part whatever they hold; a visible infinity or NaN in v gives an infinity or NaN.  0 < scale <= 2^127. */
 int cbk_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t rows, int64_t heads,
                          int64_t kv_heads, int head_dim, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                          int64_t v_row, int64_t v_head, const int32_t* cu_seqlens, int64_t num_seqs,

@@ -111,7 +111,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     0 .. i.  ``cu_seqlens`` int32 [sequences + 1] holds the sequences' first rows and the end of the last.
     ``max_seqlen`` is at least the longest sequence's length (default: all rows; a tight bound launches less).
     ``scale`` (positive, at most 2^127) defaults to head_dim ** -0.5.  Rows behind the last sequence come back as zeros, or stay as
-    they were in ``out``.  What the causal mask hides takes no part, infinities and NaN included."""
+    they were in ``out``.  What the causal mask hides takes no part, infinities and NaN included; a visible
+    infinity or NaN in v gives an infinity or NaN, whatever its weight."""
     if q.dim() != 3:
         raise ValueError("q must be [rows, heads, head_dim]")
     if scale is None:

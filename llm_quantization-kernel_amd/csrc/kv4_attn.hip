@@ -32,10 +32,10 @@
 // workgroup, by the last of its workgroups to arrive (or a second launch), in a fixed order.  Units of few blocks are not
 // cut: the workgroup that has their first block takes them whole.
 //
-// Bound: the cache's bytes, 4352 a block at D = 128 (64 sequences of 1024..8192 tokens, 8 kv heads, bf16: 245 MB in 56.5 us,
-// 4.3 TB/s of the 4.9 a large copy reaches); about 290 vector instructions a block fill a third of the issue slots.  Short
-// calls are latencies: 32 heads of one sequence of 77 tokens 5.9 us.  An even cut against a fixed number of splits a
-// sequence, 32 sequences of 64..4096 tokens: 36.4 us against 45.4.
+// Bound: the cache's bytes, 4352 a block at D = 128 (64 sequences of 1024..8192 tokens, 8 kv heads, bf16: 245 MB in 57.0 us,
+// 4.3 TB/s of the 4.9 a large copy reaches); about 320 vector instructions a block fill a third of the issue slots.  Short
+// calls are latencies: 32 heads of one sequence of 77 tokens 6.1 us.  An even cut against a fixed number of splits a
+// sequence, 32 sequences of 64..4096 tokens in fp16, with one term of w: 36.4 us against 45.4 (39.6 with two).
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
 

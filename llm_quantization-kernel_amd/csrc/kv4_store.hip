@@ -12,9 +12,9 @@
 // values each, and write one word each; the next four tokens' loads are under way meanwhile.  V's words hold eight
 // tokens of one value: the codes pass through LDS as bytes [value][token], and a word is two dwords of them folded
 // together.  A block that is not all new keeps the other tokens' codes (read ahead of the rest).
-// Bound: the bytes (the 16-bit values in, codes out; 5915 tokens of 32 heads of 128 in fp16, 123 MB: 48 us, 2.5 TB/s, the
-// vector instructions of quantizing beside it), for a decode step's tokens the latencies of table, values and old words
-// (64 tokens of 8 heads: 8 us).  The read moves as many bytes in 41 us.
+// Bound: the vector instructions of quantizing (6545 tokens of 32 heads of 128 in fp16, 136 MB with the codes: 48 us, 2.8 TB/s, 38 us of
+// vector issue), for a decode step's tokens the latencies of table, values and old words (64 tokens of 8 heads: 8 us).
+// The read moves as many bytes in 41 us.
 #include "kv4.hpp"
 #include "cbk_kernels.hpp"
 
