@@ -452,7 +452,7 @@ __global__ __launch_bounds__(64 * WAVES, kv4_waves(NS, DT) == 3 ? 3 : 1) void kv
             if constexpr (!EXACT) qsum = group_sum(qsum) * 0x1p-22f;
             // scale log2 e; for fp32 in two terms: its rounding would bend every score by 2^-24 of itself
             const int ce = UP - 11 + e + __builtin_amdgcn_frexp_expf((float)c2);
-            cc = __builtin_ldexpf(cm, ce);
+            cc = fmaxf(__builtin_ldexpf(cm, ce), 0x1p-149f);           // not zero: hidden tokens are -inf times it
             red_l[wave][n] = (float)ce;                // cc is cm 2^ce, kept there until the waves meet
             if constexpr (EXACT) cl = __builtin_ldexpf((float)(c2 - (double)(float)c2), UP - 11 + e);
         }

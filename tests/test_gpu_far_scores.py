@@ -145,3 +145,16 @@ def test_cached_large_inputs(hip, dtype):
             q = torch.zeros(2, 1, 2, d)
             q[..., 3] = a
             _cache_check(q.to(dtype), pages, page, table, ln, scale, [0, 1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size,scale", [(2.0 ** -130, 2.0 ** -30), (2.0 ** -24, 2.0 ** -140), (0.0, 2.0 ** -149), (2.0 ** -133, 2.0 ** -149)])
+def test_cached_scores_of_nothing(hip, dtype, size, scale):
+    """Queries and scales whose factor is below the smallest float: an even softmax, with hidden tokens in every block."""
+    lens, d, page = [1, 20, 45], 64, 32
+    g = torch.Generator().manual_seed(13)
+    n = sum(lens)
+    k, v = torch.randn(n, 1, d, generator=g), torch.randn(n, 1, d, generator=g)
+    pages, table, ln = _cache(lens, k, v, page)
+    q = (torch.randn(3, 1, 2, d, generator=g).sign().double() * size).to(dtype)
+    _cache_check(q, pages, page, table, ln, scale, [0, 1])
