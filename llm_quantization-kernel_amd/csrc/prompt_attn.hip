@@ -10,8 +10,7 @@
 // largest score exceeds it by 8 (w <= 2^8 then, 2^15 in fp16, in range; sums are fp32), and stays a whole number, so that what it
 // scales is exact.  w is rounded to the type (nearest even), as the products take both operands in V's type: that adds as much to
 // an output's error as its own rounding (bf16 2.3e-3 against 1.6e-3, fp16 2.9e-4 against 2.0e-4); a second term would be half
-// as many products again, of a kernel bound by them.  l sums w unrounded: taking each back from its pair would cost two more
-// instructions a pair.
+// as many products again, of a kernel bound by them.  l sums the rounded w, so that the rounding cancels where values agree.
 //
 // Bound: a tile of a wave costs 32 matrix instructions of 32 cycles (D = 128) and about as many cycles of vector
 // instructions (the softmax's, the same for any D); two waves a SIMD overlap them in part.  8192 rows, 32/8 heads, bf16:
@@ -68,6 +67,18 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 template <int DT>
 __device__ __forceinline__ float half_of(uint32_t v) {
     return Dt<DT>::to_f(__builtin_bit_cast(typename Dt<DT>::S, (uint16_t)v));
+}
+
+// l plus the two values of a packed pair, in one instruction (fp32, denormals kept).
+template <int DT>
+__device__ __forceinline__ float plus_both(uint32_t pair, float l) {
+    if constexpr (DT == DT_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, pair), h2{(_Float16)1.f, (_Float16)1.f}, l, false);
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), b2{(__bf16)1.f, (__bf16)1.f}, l, false);
+    }
 }
 
 __device__ __forceinline__ f16v zero16() {
@@ -295,8 +306,9 @@ __global__ __launch_bounds__(64 * WAVES, CP == 32 ? 1 : CP == 16 ? 2 : 3) void p
             for (int j = 0; j < 16; j += 2) {
                 const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], ca, at));
                 const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], ca, at));
-                l += x + y;
-                w[2 * i + (j >> 3)][(j & 7) >> 1] = pack2<DT>(x, y);
+                const uint32_t both = pack2<DT>(x, y);
+                w[2 * i + (j >> 3)][(j & 7) >> 1] = both;
+                l = plus_both<DT>(both, l);
             }
         };
         auto sums = [&](int i) {
