@@ -8,13 +8,13 @@
 // operand layout of w for the tokens in that order, so w stays in its lane; V^T is read transposed from LDS
 // (ds_read_b64_tr_b16) in the same token order.  The running reference M of a row moves only when a tile's
 // largest score exceeds it by 8 (w <= 2^8 then, 2^15 in fp16, in range; sums are fp32), and stays a whole number, so that what it
-// scales is exact.  w is rounded to the type (nearest even), as the products take both operands in V's type: that adds as much to
-// an output's error as its own rounding (bf16 2.3e-3 against 1.6e-3, fp16 2.9e-4 against 2.0e-4); a second term would be half
-// as many products again, of a kernel bound by them.  l sums the rounded w, so that the rounding cancels where values agree.
+// scales is exact.  w is rounded to the type (nearest even), as the products take both operands in V's type: an output's
+// error is 2.1e-3 then in bf16 and 2.5e-4 in fp16, its own rounding alone 1.6e-3 and 2.0e-4; a second term would be half as many
+// products again, of a kernel bound by them.  l sums the rounded w, so that the rounding cancels where values agree.
 //
 // Bound: a tile of a wave costs 32 matrix instructions of 32 cycles (D = 128) and about as many cycles of vector
 // instructions (the softmax's, the same for any D); two waves a SIMD overlap them in part.  8192 rows, 32/8 heads, bf16:
-// 554 us, 0.99 PFLOP/s of the 1.22 that a large matrix product reaches (554 to 573 by card); three waves a SIMD (six a
+// 560 us, 0.98 PFLOP/s of the 1.22 that a large matrix product reaches (554 to 573 by card); three waves a SIMD (six a
 // workgroup) were a tenth slower.
 //
 // Masked places take no part whatever they hold: scores there are selected away, and a V tile on the diagonal
